@@ -1,0 +1,304 @@
+"""The 8-bit integer (W8A8) path against its definition in 64 bits: row quantisers, read-back, integer product, and the
+feed-forward block they make together."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, F16, F32, F64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
+FLOOR = 2.0 ** -120
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(shape, seed, dtype=F32):
+    return torch.randn(shape, generator=_gen(seed), device="cuda").to(dtype)
+
+
+def _codes(rows, k, seed):
+    from velogb10_b200.quant import codec
+    return codec.rows16(torch.randint(-127, 128, (rows, k), generator=_gen(seed), device="cuda").to(torch.int8))
+
+
+def _check_rows(act, y, n, rel, err):
+    """``act`` holds the quantised rows ``y`` (fp64). ``rel`` bounds the relative error of a value the kernel quantised
+    (and so of the scale, plus its own two roundings); a code is off by half a step, plus that error in steps."""
+    from velogb10_b200.ops import lib
+    torch.cuda.synchronize()
+    lib.check_err_word()
+    s = (y.abs().amax(-1) / 127).clamp_min(FLOOR)
+    got = act.scale[:n].double()
+    assert ((got - s).abs() <= (rel + 2 * 2.0 ** -24) * s).all(), err
+    off = (act.q[:n].double() * got[:, None] - y).abs() / got[:, None]
+    assert off.max().item() <= 0.5 + 127 * (2 * rel + 4 * 2.0 ** -24), (err, off.max().item())
+    assert (act.q[:n].abs().amax(-1) <= 127).all()
+
+
+# every width class: one element, odd, below a vector, one CTA with one / two groups a thread, clusters of 2, 4 and 8
+WIDTHS = [1, 7, 8, 255, 512, 4111, 5120, 8192, 8200, 16384, 17408, 17411, 40000, 131071]
+
+
+@pytest.mark.parametrize("k", WIDTHS)
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+def test_quantise_rows(k, dtype):
+    from velogb10_b200.ops import int8 as I8
+    for n in (1, 5):
+        x = _randn((n, k), k + n, dtype)
+        _check_rows(I8.quantize_act_int8(x), x.double(), n, 0.0, (k, n))
+
+
+@pytest.mark.parametrize("k", WIDTHS)
+def test_swiglu_rows(k):
+    from velogb10_b200.ops import int8 as I8
+    for n in (1, 3):
+        gu = (_randn((n, 2 * k), 3 * k + n) * 3).to(BF)
+        g, u = gu[:, :k].double(), gu[:, k:].double()
+        # e^-g to 2 + 1.173 |g| ulp (|g| < 20 here: 26 * 2^-23), quotient 2 ulp, two products
+        _check_rows(I8.swiglu_int8(gu), g * torch.sigmoid(g) * u, n, 30 * 2.0 ** -23, (k, n))
+
+
+@pytest.mark.parametrize("h", WIDTHS)
+@pytest.mark.parametrize("delta,plus_one,f16", [(True, True, True), (False, False, False), (True, False, False), (False, True, True)])
+def test_add_rmsnorm_rows(h, delta, plus_one, f16):
+    from velogb10_b200.ops import int8 as I8
+    for n in (1, 4):
+        res, d = _randn((n, h), h + n, BF), _randn((n, h), 7 * h + n, BF) if delta else None
+        w = _randn((h,), 11 * h) * 0.2 + (0.0 if plus_one else 1.0)
+        out16 = torch.empty((n, h), dtype=F16, device="cuda") if f16 else None
+        want = (res.double() + d.double()).to(BF) if delta else res.clone()
+        act = I8.add_rmsnorm_int8(res, d, w, 1e-6, out16=out16, plus_one=plus_one)
+        x = want.double()
+        y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6) * (w.double() + (1.0 if plus_one else 0.0))
+        # sum of squares: 16 terms a thread, 5 + 5 shuffles, 8 ranks, the square: 35 roundings, halved by the root;
+        # reciprocal root 2 ulp; mean, eps, (w + 1) and two products: 5 roundings
+        rel = (35 / 2 + 2 * 2 + 5) * 2.0 ** -24
+        _check_rows(act, y, n, rel, (h, n))
+        assert torch.equal(res, want)
+        if f16:
+            assert ((out16.double() - y).abs() <= y.abs() * (2.0 ** -11 + rel) + 2.0 ** -24).all()
+
+
+def test_rows_with_strides_and_spare_rows():
+    """Views with a pitch, an unaligned start, and buffers with more rows than are asked for."""
+    from velogb10_b200.ops import int8 as I8
+    for off, k in ((0, 512), (3, 512), (8, 509), (0, 17408)):
+        base = _randn((9, 2 * k + 40), k + off, BF)
+        x = base[:, off:off + k]
+        out = I8.act_buffers(12, k, "cuda")
+        out.q.fill_(99)
+        out.scale.fill_(-1.0)
+        I8.quantize_act_int8(x, n=7, out=out)
+        _check_rows(out, x[:7].double(), 7, 0.0, (off, k))
+        assert (out.q[7:] == 99).all() and (out.scale[7:] == -1).all()
+        gu = base[:, off:off + 2 * k]
+        act = I8.swiglu_int8(gu, n=2)
+        g, u = gu[:2, :k].double(), gu[:2, k:].double()
+        _check_rows(act, g * torch.sigmoid(g) * u, 2, 30 * 2.0 ** -23, (off, k))
+        keep = base.clone()
+        w = torch.zeros(k + 1, device="cuda")[1:]                    # 4-byte aligned weights
+        act = I8.add_rmsnorm_int8(x, x.clone(), w, 1e-6, n=3, out=out)
+        y = (x[:3].double())
+        assert torch.equal(x[:3], (keep[:3, off:off + k].float() * 2).to(BF)) and torch.equal(base[3:], keep[3:])
+        _check_rows(act, y * torch.rsqrt(y.square().mean(-1, keepdim=True) + 1e-6), 3, 27 * 2.0 ** -24, (off, k))
+        back = torch.full((9, k + 3), 5.0, dtype=F32, device="cuda")
+        I8.dequantize_act_int8(out, n=3, out=back[:, 2:2 + k])
+        assert torch.equal(back[:3, 2:2 + k], out.q[:3].float() * out.scale[:3, None])
+        assert (back[3:] == 5).all() and (back[:, :2] == 5).all() and (back[:, 2 + k:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("k", [1, 8, 33, 4096, 131071])
+def test_read_back(dtype, k):
+    from velogb10_b200.ops import int8 as I8
+    act = I8.Int8Act(_codes(3, k, k), torch.tensor([0.5, 1e-3, 700.0], device="cuda"))
+    got = I8.dequantize_act_int8(act, dtype=dtype)
+    want = act.q.float() * act.scale[:, None]
+    assert torch.equal(got, want.clamp(-65504, 65504).to(dtype) if dtype == F16 else want.to(dtype))
+
+
+def test_rows_that_are_zero_tiny_or_not_finite():
+    from velogb10_b200.models.weights import QLinear
+    from velogb10_b200.ops import int8 as I8
+    for k in (64, 67, 20000):
+        x = _randn((6, k), k)
+        x[0] = 0.0
+        x[1] *= 1e-37                                               # below the scale's floor
+        x[2, k // 2] = float("inf")
+        x[3, k - 1] = float("nan")
+        x[4] = 3e38
+        act = I8.quantize_act_int8(x)
+        assert (act.q[0] == 0).all() and float(act.scale[0]) == FLOOR
+        assert float(act.scale[1]) == FLOOR and (act.q[1].double() * FLOOR - x[1].double()).abs().max() <= 0.5001 * FLOOR
+        assert (act.q[2:4] == 0).all() and act.scale[2:4].isnan().all()
+        assert (act.q[4] == 127).all() and act.scale[4].isfinite()
+        assert I8.dequantize_act_int8(act)[2:4].isnan().all() and I8.dequantize_act_int8(act, dtype=F16)[2:4].isnan().all()
+        q = QLinear.from_dense(_randn((40, k), k + 1), "int8")
+        out = I8.linear_int8(q, act, out_f32=True)
+        # row 4 is 3e38 * (the sum of a weight row): beyond fp32 (3.4e38) as soon as that sum exceeds 1.13
+        ref = act.scale[4].double() * 127 * q.codes.double().sum(-1) * q.row_scale.double()
+        assert torch.equal(out[4].isinf(), ref.abs() > 3.4028235e38) and not out[4].isnan().any()
+        assert (out[0] == 0).all() and out[2:4].isnan().all() and out[5].isfinite().all() and out[:2].isfinite().all()
+        gu = torch.zeros((3, 2 * k), dtype=BF, device="cuda")
+        gu[0, :k], gu[0, k:] = -1e4, 1.0                             # silu underflows to zero
+        gu[1, 0], gu[1, k:] = float("-inf"), 1.0
+        gu[2, 0], gu[2, k] = 300.0, 2.0
+        act = I8.swiglu_int8(gu)
+        assert (act.q[0] == 0).all() and float(act.scale[0]) == FLOOR
+        assert act.scale[1].isnan() and (act.q[1] == 0).all()
+        assert int(act.q[2, 0]) == 127 and (act.q[2, 1:] == 0).all() and abs(float(act.scale[2]) - 600 / 127) < 1e-4
+        res = torch.zeros((4, k), dtype=BF, device="cuda")
+        res[1, 3] = float("nan")
+        res[2] = 3e38                                                # the sum of squares leaves fp32
+        res[3, 5] = float("inf")
+        out16 = torch.empty((4, k), dtype=F16, device="cuda")
+        act = I8.add_rmsnorm_int8(res, None, torch.zeros(k, device="cuda"), 1e-6, out16=out16)
+        assert (act.q == 0).all() and float(act.scale[0]) == FLOOR and act.scale[1:].isnan().all()
+        assert (out16[0] == 0).all() and out16[1:].isnan().all()
+
+
+def _product(q, act, n, out_f32, m=None):
+    from velogb10_b200.ops import int8 as I8, lib
+    got = I8.linear_int8(q, act, n=n, out_f32=out_f32)
+    torch.cuda.synchronize()
+    lib.check_err_word()
+    ref = (act.q[:n].double() @ q.codes.double().t()) * act.scale[:n].double()[:, None] * q.row_scale.double()
+    # exact sum; its conversion and two products round to fp32, the store to bf16
+    tol = 3.1 * 2.0 ** -24 + (0.0 if out_f32 else 2.0 ** -8)
+    assert ((got.double() - ref).abs() <= tol * ref.abs()).all(), (q.m, q.k, n)
+    return got
+
+
+def _weights(m, k, seed):
+    from velogb10_b200.models.weights import QLinear
+    return QLinear("int8", m, k, codes=_codes(m, k, seed), row_scale=0.01 * (1 + torch.rand(m, generator=_gen(seed), device="cuda")))
+
+
+def _tokens(n, k, seed):
+    from velogb10_b200.ops import int8 as I8
+    return I8.Int8Act(_codes(n, k, seed), 0.02 * (1 + torch.rand(n, generator=_gen(seed), device="cuda")))
+
+
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 128), (5, 17), (128, 127), (129, 129), (1001, 2063), (256, 8192), (640, 5120),
+                                 (5120, 1024), (2000, 4160)])
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 32, 33, 63, 65, 128, 129, 255, 256, 257, 511, 700, 1111])
+def test_product(m, k, n):
+    _product(_weights(m, k, m + k), _tokens(n, k, n), n, (m + n) % 2 == 0)
+
+
+@pytest.mark.parametrize("m,k,n", [(34816, 5120, 1), (5120, 17408, 16), (34816, 5120, 300), (5120, 17408, 2048), (100000, 512, 7),
+                                   (8192, 256, 4096), (131, 64, 70000)])
+def test_product_at_model_widths(m, k, n):
+    _product(_weights(m, k, 1), _tokens(n, k, 2), n, False)
+
+
+def test_product_extremes_do_not_overflow():
+    """Every code at its limit over the longest sum: 128 * 128 * 131071 fits 32 bits."""
+    from velogb10_b200.models.weights import QLinear
+    from velogb10_b200.ops import int8 as I8
+    k = I8.MAX_K
+    for n in (1, 40, 300):
+        q, act = _weights(130, k, 3), _tokens(n, k, 4)
+        q.codes.fill_(-128)
+        act.q.fill_(-128)
+        q.codes[1::2] = 127
+        _product(q, act, n, True)
+        assert float(I8.linear_int8(q, act, out_f32=True)[0, 0]) > 0 > float(I8.linear_int8(q, act, out_f32=True)[0, 1])
+
+
+def test_product_does_not_depend_on_the_batch():
+    from velogb10_b200.ops import int8 as I8
+    for m, k in ((5120, 4160), (1001, 2063), (300, 300)):
+        q, act = _weights(m, k, 5), _tokens(1030, k, 6)
+        whole = I8.linear_int8(q, act)
+        for n in (1, 3, 16, 17, 50, 128, 200, 257, 600):
+            assert torch.equal(I8.linear_int8(q, act, n=n), whole[:n]), (m, k, n)
+        one = I8.linear_int8(q, I8.Int8Act(act.q[1029:], act.scale[1029:]))
+        assert torch.equal(one[0], whole[1029])
+        assert torch.equal(I8.linear_int8(q, act), whole)
+
+
+def test_product_into_views_leaves_the_rest_alone():
+    from velogb10_b200.ops import int8 as I8
+    for m, k, n in ((200, 64, 3), (129, 300, 20), (1000, 512, 290)):
+        q, act = _weights(m, k, 7), _tokens(n + 5, k, 8)
+        for dtype in (BF, F32):
+            buf = torch.full((n + 4, m + 9), 3.0, dtype=dtype, device="cuda")
+            view = buf[1:, 5:5 + m]
+            I8.linear_int8(q, act, n=n, out=view)
+            assert torch.equal(view[:n], I8.linear_int8(q, act, n=n, out_f32=dtype == F32))
+            buf[1:n + 1, 5:5 + m] = 3.0
+            assert (buf == 3).all()
+        # wide pitches on the inputs
+        wide = torch.zeros((m, 2 * ((k + 15) // 16 * 16)), dtype=torch.int8, device="cuda")
+        wide[:, :k] = q.codes
+        q2 = type(q)("int8", m, k, codes=wide[:, :k], row_scale=q.row_scale)
+        assert torch.equal(I8.linear_int8(q2, act, n=n), I8.linear_int8(q, act, n=n))
+
+
+def test_no_rows():
+    from velogb10_b200.ops import int8 as I8
+    act = I8.quantize_act_int8(torch.zeros((0, 64), device="cuda"))
+    assert act.q.shape == (0, 64) and I8.linear_int8(_weights(8, 64, 0), act).shape == (0, 8)
+    assert I8.dequantize_act_int8(act).shape == (0, 64)
+    assert I8.swiglu_int8(torch.zeros((4, 64), dtype=BF, device="cuda"), n=0).q.shape == (0, 32)
+
+
+def _block(res, delta, w, gate_up, down):
+    from velogb10_b200.ops import int8 as I8
+    act = I8.add_rmsnorm_int8(res, delta, w, 1e-6)
+    act = I8.swiglu_int8(I8.linear_int8(gate_up, act))
+    return I8.linear_int8(down, act)
+
+
+@pytest.mark.parametrize("n,h,inter", [(1, 256, 512), (16, 2048, 512), (33, 640, 1111), (300, 1000, 776)])
+def test_feed_forward_block(n, h, inter):
+    """The operators as a decoder layer runs them, on their own stream and as a replayed graph: the same bits."""
+    from velogb10_b200.models.weights import QLinear
+    from velogb10_b200.ops import lib
+    gate_up = QLinear.from_dense(_randn((2 * inter, h), 1) / h ** 0.5, "int8")
+    down = QLinear.from_dense(_randn((h, inter), 2) / inter ** 0.5, "int8")
+    w, res, delta = _randn((h,), 3) * 0.1, _randn((n, h), 4, BF), _randn((n, h), 5, BF)
+    res0 = res.clone()
+    out = _block(res, delta, w, gate_up, down)
+    torch.cuda.synchronize()
+    lib.check_err_word()
+    # the same definition in 64 bits, rounded where the operators store bf16
+    x = (res0.double() + delta.double()).to(BF).double()
+    assert torch.equal(res.double(), x)
+    y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6) * (1 + w.double())
+
+    def quantised(y, q):
+        s = (y.abs().amax(-1, keepdim=True) / 127)
+        return torch.round(y / s) * s @ (q.codes.double() * q.row_scale.double()[:, None]).t()
+
+    gu = quantised(y, gate_up).to(BF).double()
+    g, u = gu[:, :inter], gu[:, inter:]
+    ref = quantised(g * torch.sigmoid(g) * u, down)
+    # a code that falls on the other side of a tie moves a value by one step (1 / 127 of the row's largest) in a few
+    # places out of k: far below the rounding of the bf16 output, which is 2^-8 of each value
+    assert ((out.double() - ref).norm() / ref.norm()).item() <= 2.0 ** -8
+    # another stream
+    res2, side = res0.clone(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out2 = _block(res2, delta, w, gate_up, down)
+    side.synchronize()
+    assert torch.equal(out2, out) and torch.equal(res2, res)
+    # two captured graphs that share nothing, replayed on changed inputs
+    res3, res4 = res0.clone(), res0.clone()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        out3 = _block(res3, delta, w, gate_up, down)
+    with torch.cuda.graph(g2):
+        out4 = _block(res4, delta, w, gate_up, down)
+    res3.copy_(res0)
+    res4.copy_(res0 * 2)
+    g1.replay()
+    g2.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out3, out) and torch.equal(res3, res)
+    res5 = res0 * 2
+    assert torch.equal(out4, _block(res5, delta, w, gate_up, down)) and torch.equal(res4, res5)
+    lib.check_err_word()

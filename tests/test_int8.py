@@ -1,0 +1,113 @@
+"""The 8-bit integer path on the host: weight codec, containers, and the refusals of the wrappers (all of them before
+anything is enqueued)."""
+import pytest
+import torch
+
+from velogb10_b200.models.weights import QLinear, fuse_rows
+from velogb10_b200.ops import int8 as I8
+from velogb10_b200.ops.lib import KernelError
+from velogb10_b200.quant import codec
+
+
+@pytest.mark.parametrize("m,k", [(1, 1), (5, 16), (64, 33), (200, 515)])
+def test_codec_is_within_half_a_step(m, k):
+    g = torch.Generator().manual_seed(m * 1000 + k)
+    w = torch.randn(m, k, generator=g)
+    q = codec.quantize_int8(w)
+    assert q.codes.dtype == torch.int8 and q.codes.shape == (m, k)
+    assert q.codes.data_ptr() % 16 == 0 and (m == 1 or q.codes.stride(0) % 16 == 0)
+    assert torch.equal(q.row_scale, w.abs().amax(-1) / 127.0)
+    assert (q.codes.abs().amax(-1) == 127).all()
+    # half a step, plus the roundings of the division (2^-24 of at most 127 steps) and of the scale
+    off = (q.codes.double() * q.row_scale.double()[:, None] - w.double()).abs() / q.row_scale.double()[:, None]
+    assert off.max() <= 0.5 + 127 * 2 * 2.0 ** -24
+    assert torch.equal(codec.dequantize_int8(q.codes, q.row_scale, torch.float32), q.codes.float() * q.row_scale[:, None])
+
+
+def test_zero_rows_and_fake_quant():
+    w = torch.zeros(3, 20)
+    w[1] = torch.arange(20.0) - 10
+    q = codec.quantize_int8(w)
+    assert (q.codes[0] == 0).all() and (q.codes[2] == 0).all() and float(q.row_scale[0]) == 2.0 ** -120
+    assert (codec.fake_quant(w, "int8") - w).abs().max() <= 10 / 127 / 2 * 1.0001
+    assert codec.bits_per_weight("int8", 32) == 9.0
+
+
+def test_container_keeps_rows_on_16_byte_boundaries():
+    g = torch.Generator().manual_seed(0)
+    w = torch.randn(24, 50, generator=g)
+    q = QLinear.from_dense(w, "int8")
+    assert q.fmt == "int8" and q.codes.stride(0) == 64 and torch.equal(q.dequant(), q.codes.float() * q.row_scale[:, None])
+    two = fuse_rows([q, q])
+    assert two.m == 48 and torch.equal(two.codes[24:], q.codes) and two.codes.stride(0) % 16 == 0
+    part = q.rows(3, 9)
+    assert torch.equal(part.codes, q.codes[3:9]) and part.codes.stride(0) % 16 == 0 and torch.equal(part.row_scale, q.row_scale[3:9])
+    cut = q.cols(16, 48)
+    assert torch.equal(cut.codes, q.codes[:, 16:48]) and cut.codes.stride(0) % 16 == 0
+    assert q.to("cpu").codes.stride(0) % 16 == 0
+    mixed = fuse_rows([q, QLinear.from_dense(w, "fp8")])
+    assert mixed.fmt == "bf16"
+
+
+def _act(n, k):
+    return I8.Int8Act(codec.rows16(torch.zeros((n, k), dtype=torch.int8)), torch.ones(n))
+
+
+def _w(m, k):
+    return QLinear("int8", m, k, codes=codec.rows16(torch.zeros((m, k), dtype=torch.int8)), row_scale=torch.ones(m))
+
+
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.parametrize("what,call", [
+    ("expected a matrix", lambda: I8.quantize_act_int8(torch.zeros(8))),
+    ("not supported", lambda: I8.quantize_act_int8(torch.zeros(2, 8, dtype=torch.float64))),
+    ("rows asked for", lambda: I8.quantize_act_int8(torch.zeros(2, 8), n=3)),
+    ("rows asked for", lambda: I8.quantize_act_int8(torch.zeros(2, 8), n=-1)),
+    ("contiguous", lambda: I8.quantize_act_int8(torch.zeros(8, 2).t())),
+    ("contiguous", lambda: I8.quantize_act_int8(torch.zeros(1, 8).expand(2, 8))),
+    ("outside", lambda: I8.quantize_act_int8(torch.zeros(2, 0))),
+    ("outside", lambda: I8.quantize_act_int8(torch.zeros(1, I8.MAX_K + 1))),
+    ("out.q", lambda: I8.quantize_act_int8(torch.zeros(2, 8), out=_act(1, 8))),
+    ("out.q", lambda: I8.quantize_act_int8(torch.zeros(2, 8), out=_act(2, 9))),
+    ("out.scale", lambda: I8.quantize_act_int8(torch.zeros(2, 8), out=I8.Int8Act(_act(2, 8).q, torch.ones(1)))),
+    ("out.scale", lambda: I8.quantize_act_int8(torch.zeros(2, 8), out=I8.Int8Act(_act(2, 8).q, torch.ones(2, dtype=F16)))),
+    ("gu", lambda: I8.swiglu_int8(torch.zeros(2, 7, dtype=BF))),
+    ("gu", lambda: I8.swiglu_int8(torch.zeros(2, 8, dtype=BF), inter=3)),
+    ("gu", lambda: I8.swiglu_int8(torch.zeros(2, 8))),
+    ("eps", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), None, torch.ones(8), 0.0)),
+    ("eps", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), None, torch.ones(8), float("nan"))),
+    ("w:", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), None, torch.ones(9), 1e-6)),
+    ("w:", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), None, torch.ones(8, dtype=BF), 1e-6)),
+    ("w:", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), None, torch.ones(16)[::2], 1e-6)),
+    ("res", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8), None, torch.ones(8), 1e-6)),
+    ("delta", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), torch.zeros(1, 8, dtype=BF), torch.ones(8), 1e-6)),
+    ("delta", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), torch.zeros(2, 8), torch.ones(8), 1e-6)),
+    ("out16", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), None, torch.ones(8), 1e-6, out16=torch.zeros(2, 9, dtype=F16))),
+    ("act.q", lambda: I8.dequantize_act_int8(I8.Int8Act(torch.zeros(2, 8), torch.ones(2)))),
+    ("act.scale", lambda: I8.dequantize_act_int8(I8.Int8Act(_act(2, 8).q, torch.ones(1)))),
+    ("dtype", lambda: I8.dequantize_act_int8(_act(2, 8), dtype=torch.float64)),
+    ("out", lambda: I8.dequantize_act_int8(_act(2, 8), out=torch.zeros(2, 9))),
+    ("takes int8 weights", lambda: I8.linear_int8(QLinear.from_dense(torch.zeros(4, 16), "fp8"), _act(2, 16))),
+    ("act.q", lambda: I8.linear_int8(_w(4, 32), _act(2, 16))),
+    ("rows asked for", lambda: I8.linear_int8(_w(4, 32), _act(2, 32), n=3)),
+    ("16-byte", lambda: I8.linear_int8(_w(4, 33), I8.Int8Act(torch.zeros((2, 33), dtype=torch.int8), torch.ones(2)))),
+    ("16-byte", lambda: I8.linear_int8(_w(4, 32), I8.Int8Act(torch.zeros(80, dtype=torch.int8)[1:65].view(2, 32), torch.ones(2)))),
+    ("16-byte", lambda: I8.linear_int8(QLinear("int8", 2, 33, codes=torch.zeros((2, 33), dtype=torch.int8), row_scale=torch.ones(2)), _act(2, 33))),
+    ("row_scale", lambda: I8.linear_int8(QLinear("int8", 4, 32, codes=_w(4, 32).codes, row_scale=torch.ones(3)), _act(2, 32))),
+    ("codes", lambda: I8.linear_int8(QLinear("int8", 5, 32, codes=_w(4, 32).codes, row_scale=torch.ones(5)), _act(2, 32))),
+    ("act.scale", lambda: I8.linear_int8(_w(4, 32), I8.Int8Act(_act(2, 32).q, torch.ones(1)))),
+    ("K must be", lambda: I8.linear_int8(_w(1, I8.MAX_K + 1), _act(1, I8.MAX_K + 1))),
+    ("out", lambda: I8.linear_int8(_w(4, 32), _act(2, 32), out=torch.zeros(2, 5))),
+    ("out", lambda: I8.linear_int8(_w(4, 32), _act(2, 32), out=torch.zeros(2, 4, dtype=F16))),
+    ("out", lambda: I8.linear_int8(_w(4, 32), _act(2, 32), out=torch.zeros(4, 2).t())),
+    ("CUDA", lambda: I8.linear_int8(_w(4, 32), _act(2, 32))),
+    ("CUDA", lambda: I8.quantize_act_int8(torch.zeros(2, 8))),
+    ("CUDA", lambda: I8.swiglu_int8(torch.zeros(2, 8, dtype=BF))),
+    ("CUDA", lambda: I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), None, torch.ones(8), 1e-6)),
+    ("CUDA", lambda: I8.dequantize_act_int8(_act(2, 8))),
+])
+def test_refusals(what, call):
+    with pytest.raises(KernelError, match=what):
+        call()

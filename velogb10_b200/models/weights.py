@@ -9,6 +9,8 @@ Canonical in-memory form of a linear ``[M, K]``:
   with different global scales can be fused along M (the reference keeps one scale per 16-row tile
   for the same purpose, reference: src/quant.rs:597-633).
 * ``fp8``: ``codes`` u8 [M, K], ``row_scale`` f32 [M].
+* ``int8``: ``codes`` int8 [M, K] (rows on 16-byte boundaries), ``row_scale`` f32 [M]; read as they are by
+  ``velogb10_b200.ops.int8`` together with int8 activations.
 * ``bf16``: ``w`` bf16 [M, K].
 
 The kernel-side tile-major layout is derived from this form by ``velogb10_b200.ops.gemm``.
@@ -56,6 +58,9 @@ class QLinear:
         if fmt == "fp8":
             q8 = codec.quantize_fp8(w2)
             return cls("fp8", m, k, codes=q8.codes, row_scale=q8.row_scale, experts=experts)
+        if fmt == "int8":
+            qi = codec.quantize_int8(w2)
+            return cls("int8", m, k, codes=qi.codes, row_scale=qi.row_scale, experts=experts)
         return cls("bf16", m, k, w=w2.to(torch.bfloat16).contiguous(), experts=experts)
 
     # -- math
@@ -67,19 +72,25 @@ class QLinear:
             return v.reshape(self.m, self.k).to(dtype)
         if self.fmt == "fp8":
             return (codec.e4m3_decode(self.codes) * self.row_scale.unsqueeze(-1)).to(dtype)
+        if self.fmt == "int8":
+            return codec.dequantize_int8(self.codes, self.row_scale, dtype)
         return self.w.to(dtype)
 
     def to(self, device) -> "QLinear":
         def mv(t):
             return None if t is None else t.to(device)
-        return QLinear(self.fmt, self.m, self.k, mv(self.packed), mv(self.scales), mv(self.codes),
+        codes = mv(self.codes)
+        if self.fmt == "int8":
+            codes = codec.rows16(codes)
+        return QLinear(self.fmt, self.m, self.k, mv(self.packed), mv(self.scales), codes,
                        mv(self.row_scale), mv(self.w), None, self.experts)
 
     # -- slicing (tensor parallel)
     def rows(self, r0: int, r1: int) -> "QLinear":
         def sl(t):
             return None if t is None else t[r0:r1].contiguous()
-        return QLinear(self.fmt, r1 - r0, self.k, sl(self.packed), sl(self.scales), sl(self.codes),
+        codes = codec.rows16(sl(self.codes)) if self.fmt == "int8" else sl(self.codes)
+        return QLinear(self.fmt, r1 - r0, self.k, sl(self.packed), sl(self.scales), codes,
                        sl(self.row_scale), sl(self.w), None, 1)
 
     def cols(self, k0: int, k1: int) -> "QLinear":
@@ -90,6 +101,8 @@ class QLinear:
             q.scales = self.scales[:, k0 // 16:k1 // 16].contiguous()
         elif self.fmt == "fp8":
             q.codes = self.codes[:, k0:k1].contiguous()
+        elif self.fmt == "int8":
+            q.codes = codec.rows16(self.codes[:, k0:k1].contiguous())
         else:
             q.w = self.w[:, k0:k1].contiguous()
         return q
@@ -132,6 +145,8 @@ def fuse_rows(parts: List[QLinear]) -> QLinear:
         return QLinear(fmt, m, k, packed=cat("packed"), scales=cat("scales"), row_scale=cat("row_scale"))
     if fmt == "fp8":
         return QLinear(fmt, m, k, codes=cat("codes"), row_scale=cat("row_scale"))
+    if fmt == "int8":
+        return QLinear(fmt, m, k, codes=codec.rows16(cat("codes")), row_scale=cat("row_scale"))
     return QLinear(fmt, m, k, w=cat("w"))
 
 

@@ -1,0 +1,208 @@
+"""The 8-bit integer (W8A8) linear path: row quantisers that feed it and the integer matrix product.
+
+A token row ``y`` becomes int8 codes with one fp32 scale, ``s = max(max|y| / 127, 2^-120)``, ``q = rint(y / s)``; a weight
+row (output channel) likewise, once, at load (``codec.quantize_int8``, ``QLinear.from_dense(w, "int8")``). The product
+``out[i, m] = (sum_k q[i, k] c[m, k]) * s[i] * row_scale[m]`` has an exact integer sum, so it depends neither on the batch
+width nor on how the kernel splits K.
+
+A row that holds an infinity or a NaN gets scale NaN and codes 0: all that is computed from it is NaN.
+
+Wrappers check their arguments before anything is enqueued (``KernelError``), launch on the current stream of the
+tensors' device, and allocate only what the caller does not hand in. Rows ``>= n`` of every buffer stay as they are.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from ..models.weights import QLinear
+from . import lib as _lib
+from .lib import KernelError, c_float, c_int, c_ll, c_void_p
+
+MAX_K = 131071                 # 128 * 128 * K must stay below 2^31
+MAX_ROWS = 1 << 27
+_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+@dataclass
+class Int8Act:
+    """Quantised tokens: ``q`` int8 ``[rows, k]`` (row pitch a multiple of 16 bytes), ``scale`` fp32 ``[rows]``."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+def act_buffers(rows: int, k: int, device) -> Int8Act:
+    """Buffers a quantiser can write into (``out=``) and ``linear_int8`` can read."""
+    kp = (k + 15) & ~15
+    q = torch.empty((rows, kp), dtype=torch.int8, device=device)
+    return Int8Act(q if kp == k else q[:, :k], torch.empty((rows,), dtype=torch.float32, device=device))
+
+
+_fns = {}
+
+
+def _fn(name: str):
+    """C entry with its argument types set once (plain ints and floats then convert without wrapper objects)."""
+    f = _fns.get(name)
+    if f is None:
+        P, I, L, F = c_void_p, c_int, c_ll, c_float
+        types = {"vg_quant_int8": (P, L, I, I, I, P, L, P, P),
+                 "vg_swiglu_int8": (P, L, I, I, P, L, P, P),
+                 "vg_add_rmsnorm_int8": (P, L, P, L, P, I, I, F, I, P, L, P, P, L, P),
+                 "vg_dequant_int8": (P, L, P, P, L, I, I, I, P),
+                 "vg_gemm_int8": (P, L, P, P, L, P, P, L, I, I, I, I, P, P)}[name]
+        f = getattr(_lib.lib(), name)
+        f.argtypes = types
+        f.restype = c_int
+        _fns[name] = f
+    return f
+
+
+def _launch(name: str, device: torch.device, *args):
+    if device.type != "cuda":
+        raise KernelError(f"{name[3:]} runs on CUDA tensors, got {device}")
+    if device.index == torch.cuda.current_device():
+        _lib.check(_fn(name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        return
+    with torch.cuda.device(device):
+        _lib.check(_fn(name)(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+def _matrix(t: torch.Tensor, what: str, dtypes, rows: int, cols: int, device=None) -> int:
+    """Row pitch of a 2-D row-major argument that has to hold ``rows`` x ``cols`` elements."""
+    if t.dtype not in dtypes:
+        raise KernelError(f"{what}: dtype {t.dtype} is not supported")
+    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] != cols:
+        raise KernelError(f"{what}: shape {tuple(t.shape)}, expected at least {rows} rows of {cols}")
+    if device is not None and t.device != device:
+        raise KernelError(f"{what} is on {t.device}, expected {device}")
+    ld, inner = t.stride()
+    if (inner != 1 and cols > 1) or (ld < cols and rows > 1):
+        raise KernelError(f"{what}: rows must be contiguous and must not overlap (strides {t.stride()})")
+    return ld if rows > 1 else max(ld, cols)
+
+
+def _rows(t: torch.Tensor, n: Optional[int], what: str) -> int:
+    if t.dim() != 2:
+        raise KernelError(f"{what}: expected a matrix, got shape {tuple(t.shape)}")
+    n = t.shape[0] if n is None else n
+    if n < 0 or n > t.shape[0] or n > MAX_ROWS:
+        raise KernelError(f"{what}: {n} rows asked for, the tensor has {t.shape[0]}")
+    return n
+
+
+def _vector(t: torch.Tensor, what: str, size: int, device, least: bool = False):
+    if t.dtype != torch.float32 or t.dim() != 1 or (t.shape[0] < size if least else t.shape[0] != size) or t.device != device \
+            or (t.stride(0) != 1 and t.shape[0] > 1):
+        raise KernelError(f"{what}: expected {size} contiguous fp32 values on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _out(out: Optional[Int8Act], n: int, k: int, device):
+    """The quantisers' output buffers and their row pitch."""
+    if k < 1 or k > MAX_K:
+        raise KernelError(f"row width {k} is outside 1 .. {MAX_K}")
+    if out is None:
+        out = act_buffers(n, k, device)
+        return out, (k + 15) & ~15
+    ld = _matrix(out.q, "out.q", (torch.int8,), n, k, device)
+    _vector(out.scale, "out.scale", n, device, least=True)
+    return out, ld
+
+
+def quantize_act_int8(x: torch.Tensor, n: Optional[int] = None, out: Optional[Int8Act] = None) -> Int8Act:
+    """Quantise rows ``x[:n]`` (bf16 / f16 / f32 ``[rows, k]``)."""
+    n = _rows(x, n, "x")
+    k, dev = x.shape[1], x.device
+    out, ldq = _out(out, n, k, dev)
+    ld = _matrix(x, "x", _DTYPE, n, k)
+    if n:
+        _launch("vg_quant_int8", dev, x.data_ptr(), ld, _DTYPE[x.dtype], n, k, out.q.data_ptr(), ldq, out.scale.data_ptr())
+    return out
+
+
+def swiglu_int8(gu: torch.Tensor, n: Optional[int] = None, inter: Optional[int] = None, out: Optional[Int8Act] = None) -> Int8Act:
+    """``silu(gate) * up`` of ``gu[:n] = [gate | up]`` (bf16 ``[rows, 2 * inter]``), quantised."""
+    n = _rows(gu, n, "gu")
+    if inter is None:
+        inter = gu.shape[1] // 2
+    ld = _matrix(gu, "gu", (torch.bfloat16,), n, 2 * inter)
+    out, ldq = _out(out, n, inter, gu.device)
+    if n:
+        _launch("vg_swiglu_int8", gu.device, gu.data_ptr(), ld, n, inter, out.q.data_ptr(), ldq, out.scale.data_ptr())
+    return out
+
+
+def add_rmsnorm_int8(res: torch.Tensor, delta: Optional[torch.Tensor], w: torch.Tensor, eps: float, n: Optional[int] = None,
+                     out: Optional[Int8Act] = None, out16: Optional[torch.Tensor] = None, plus_one: bool = True) -> Int8Act:
+    """``res[:n] += delta[:n]`` (bf16, in place, when delta is given), then RMSNorm with weights ``w`` (``1 + w`` with
+    ``plus_one``) quantised; the normed rows also go to ``out16`` (f16, saturating) when it is given."""
+    n = _rows(res, n, "res")
+    h, dev = res.shape[1], res.device
+    if not eps > 0.0:
+        raise KernelError(f"eps must be positive, got {eps}")
+    out, ldq = _out(out, n, h, dev)
+    ld = _matrix(res, "res", (torch.bfloat16,), n, h)
+    ldd = ldo = 0
+    if delta is not None:
+        ldd = _matrix(delta, "delta", (torch.bfloat16,), n, h, dev)
+    if out16 is not None:
+        ldo = _matrix(out16, "out16", (torch.float16,), n, h, dev)
+    _vector(w, "w", h, dev)
+    if n:
+        _launch("vg_add_rmsnorm_int8", dev, res.data_ptr(), ld, 0 if delta is None else delta.data_ptr(), ldd, w.data_ptr(), n, h,
+                eps, 1 if plus_one else 0, out.q.data_ptr(), ldq, out.scale.data_ptr(),
+                0 if out16 is None else out16.data_ptr(), ldo)
+    return out
+
+
+def dequantize_act_int8(act: Int8Act, n: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                        dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values rows ``act.q[:n]`` stand for, in bf16, f16 (saturating) or f32 (``out``'s type when it is given)."""
+    n = _rows(act.q, n, "act.q")
+    k, dev = act.q.shape[1], act.q.device
+    if k < 1 or k > MAX_K:
+        raise KernelError(f"row width {k} is outside 1 .. {MAX_K}")
+    ldq = _matrix(act.q, "act.q", (torch.int8,), n, k)
+    _vector(act.scale, "act.scale", n, dev, least=True)
+    if out is None:
+        if dtype not in _DTYPE:
+            raise KernelError(f"dtype {dtype} is not supported")
+        out = torch.empty((n, k), dtype=dtype, device=dev)
+    ldo = _matrix(out, "out", _DTYPE, n, k, dev)
+    if n:
+        _launch("vg_dequant_int8", dev, act.q.data_ptr(), ldq, act.scale.data_ptr(), out.data_ptr(), ldo, _DTYPE[out.dtype], n, k)
+    return out
+
+
+def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                out_f32: bool = False) -> torch.Tensor:
+    """``out[:n] = act @ W^T`` for an ``int8`` linear, bf16 or fp32 (``out``'s type when it is given). Codes of both sides are
+    read in place: rows must start on 16-byte boundaries (``codec.rows16`` re-lays a matrix whose rows do not)."""
+    if q.fmt != "int8":
+        raise KernelError(f"linear_int8 takes int8 weights, got {q.fmt}")
+    n = _rows(act.q, n, "act.q")
+    m, k, dev = q.m, q.k, act.q.device
+    if k < 1 or k > MAX_K or m < 1:
+        raise KernelError(f"weights [{m}, {k}]: K must be in 1 .. {MAX_K}")
+    ldw = _matrix(q.codes, "codes", (torch.int8,), m, k, dev)
+    ldq = _matrix(act.q, "act.q", (torch.int8,), n, k)
+    if m == 1:
+        ldw = (k + 15) & ~15
+    if n <= 1:
+        ldq = (k + 15) & ~15
+    wp, qp = q.codes.data_ptr(), act.q.data_ptr()
+    if (ldw | ldq | wp | qp) & 15:
+        raise KernelError("int8 rows must start on 16-byte boundaries (codec.rows16)")
+    _vector(q.row_scale, "row_scale", m, dev)
+    _vector(act.scale, "act.scale", n, dev, least=True)
+    if out is None:
+        out = torch.empty((n, m), dtype=torch.float32 if out_f32 else torch.bfloat16, device=dev)
+        ldo = m
+    else:
+        ldo = _matrix(out, "out", (torch.bfloat16, torch.float32), n, m, dev)
+    if n:
+        _launch("vg_gemm_int8", dev, wp, ldw, q.row_scale.data_ptr(), qp, ldq, act.scale.data_ptr(), out.data_ptr(), ldo,
+                1 if out.dtype == torch.float32 else 0, m, k, n, _lib.err_word(dev).data_ptr() if dev.type == "cuda" else 0)
+    return out

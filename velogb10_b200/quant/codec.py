@@ -1,4 +1,4 @@
-"""NVFP4 / FP8 weight-only codec (torch, vectorised; runs on CPU or CUDA tensors).
+"""NVFP4 / FP8 / INT8 weight codec (torch, vectorised; runs on CPU or CUDA tensors).
 
 Bit-level contract, identical to the reference codec (reference: src/quant.rs:37-275):
 
@@ -10,6 +10,7 @@ Bit-level contract, identical to the reference codec (reference: src/quant.rs:37
   convention (dequant divides by it), block scale ``e4m3(amax(block)/6/s_tensor)``, packed two
   codes per byte with the low nibble holding the even index.
 * FP8: one f32 scale per output row (``amax/448``), codes are E4M3.
+* INT8 (not in the reference): one f32 scale per output row (``amax/127``), symmetric codes, round half to even.
 """
 from __future__ import annotations
 
@@ -166,6 +167,43 @@ def dequantize_fp8(codes: torch.Tensor, row_scale: torch.Tensor, dtype=torch.bfl
     return (e4m3_decode(codes) * row_scale.float().unsqueeze(-1)).to(dtype)
 
 
+# ------------------------------------------------------------------ INT8 per-row
+
+@dataclass
+class Int8Tensor:
+    codes: torch.Tensor      # [M, K] int8, rows on 16-byte boundaries
+    row_scale: torch.Tensor  # [M] f32
+    m: int
+    k: int
+
+
+def rows16(codes: torch.Tensor) -> torch.Tensor:
+    """The same int8 matrix with every row on a 16-byte boundary, as the tensor copies of the integer product need it
+    (a view into wider rows where K is not a multiple of 16; the input itself where it already fits)."""
+    assert codes.dtype == torch.int8 and codes.dim() == 2
+    m, k = codes.shape
+    if codes.data_ptr() % 16 == 0 and codes.stride(1) == 1 and codes.stride(0) % 16 == 0 and codes.stride(0) >= k:
+        return codes
+    t = torch.zeros((m, (k + 15) // 16 * 16), dtype=torch.int8, device=codes.device)[:, :k]
+    return t.copy_(codes)
+
+
+def quantize_int8(w: torch.Tensor, row_chunk: int = 8192) -> Int8Tensor:
+    m, k = w.shape
+    codes = rows16(torch.empty((m, k), dtype=torch.int8, device=w.device))
+    row_scale = torch.empty((m,), dtype=torch.float32, device=w.device)
+    for r0 in range(0, m, row_chunk):
+        x = w[r0:r0 + row_chunk].float()
+        s = (x.abs().amax(dim=-1) / 127.0).clamp_min(2.0 ** -120)
+        row_scale[r0:r0 + row_chunk] = s
+        codes[r0:r0 + row_chunk] = torch.round(x / s.unsqueeze(-1)).clamp_(-127, 127).to(torch.int8)
+    return Int8Tensor(codes, row_scale, m, k)
+
+
+def dequantize_int8(codes: torch.Tensor, row_scale: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    return (codes.float() * row_scale.float().unsqueeze(-1)).to(dtype)
+
+
 # ------------------------------------------------------------------ helpers
 
 def fake_quant(w: torch.Tensor, fmt: str) -> torch.Tensor:
@@ -179,13 +217,16 @@ def fake_quant(w: torch.Tensor, fmt: str) -> torch.Tensor:
     elif fmt == "fp8":
         q8 = quantize_fp8(w2)
         out = dequantize_fp8(q8.codes, q8.row_scale, w.dtype)
+    elif fmt == "int8":
+        qi = quantize_int8(w2)
+        out = dequantize_int8(qi.codes, qi.row_scale, w.dtype)
     else:
         raise ValueError(fmt)
     return out.reshape(w.shape)
 
 
 def bits_per_weight(fmt: str, k: int) -> float:
-    return {"bf16": 16.0, "fp8": 8.0 + 32.0 / k, "nvfp4": 4.0 + 8.0 / BLOCK}[fmt]
+    return {"bf16": 16.0, "fp8": 8.0 + 32.0 / k, "int8": 8.0 + 32.0 / k, "nvfp4": 4.0 + 8.0 / BLOCK}[fmt]
 
 
 def roundtrip_error(orig: torch.Tensor, deq: torch.Tensor) -> Tuple[float, float]:
