@@ -61,21 +61,34 @@ def _fn(name: str):
 
 
 def _launch(name: str, device: torch.device, *args):
-    if device.type != "cuda":
+    index = device.index
+    if index is None or device.type != "cuda":
         raise KernelError(f"{name[3:]} runs on CUDA tensors, got {device}")
-    if device.index == torch.cuda.current_device():
-        _lib.check(_fn(name)(*args, torch.cuda.current_stream().cuda_stream), name)
+    if index == torch.cuda.current_device():
+        _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name)
         return
-    with torch.cuda.device(device):
-        _lib.check(_fn(name)(*args, torch.cuda.current_stream().cuda_stream), name)
+    with torch.cuda.device(index):
+        _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name)
+
+
+def _rows(t: torch.Tensor, n: Optional[int], what: str) -> int:
+    if t.dim() != 2:
+        raise KernelError(f"{what}: expected a matrix, got shape {tuple(t.shape)}")
+    rows = t.shape[0]
+    if n is None:
+        n = rows
+    if not 0 <= n <= rows or n > MAX_ROWS:
+        raise KernelError(f"{what}: {n} rows asked for, the tensor has {rows}")
+    return n
 
 
 def _matrix(t: torch.Tensor, what: str, dtypes, rows: int, cols: int, device=None) -> int:
     """Row pitch of a 2-D row-major argument that has to hold ``rows`` x ``cols`` elements."""
     if t.dtype not in dtypes:
         raise KernelError(f"{what}: dtype {t.dtype} is not supported")
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] != cols:
-        raise KernelError(f"{what}: shape {tuple(t.shape)}, expected at least {rows} rows of {cols}")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] < rows or shape[1] != cols:
+        raise KernelError(f"{what}: shape {tuple(shape)}, expected at least {rows} rows of {cols}")
     if device is not None and t.device != device:
         raise KernelError(f"{what} is on {t.device}, expected {device}")
     ld, inner = t.stride()
@@ -84,18 +97,9 @@ def _matrix(t: torch.Tensor, what: str, dtypes, rows: int, cols: int, device=Non
     return ld if rows > 1 else max(ld, cols)
 
 
-def _rows(t: torch.Tensor, n: Optional[int], what: str) -> int:
-    if t.dim() != 2:
-        raise KernelError(f"{what}: expected a matrix, got shape {tuple(t.shape)}")
-    n = t.shape[0] if n is None else n
-    if n < 0 or n > t.shape[0] or n > MAX_ROWS:
-        raise KernelError(f"{what}: {n} rows asked for, the tensor has {t.shape[0]}")
-    return n
-
-
 def _vector(t: torch.Tensor, what: str, size: int, device, least: bool = False):
-    if t.dtype != torch.float32 or t.dim() != 1 or (t.shape[0] < size if least else t.shape[0] != size) or t.device != device \
-            or (t.stride(0) != 1 and t.shape[0] > 1):
+    if t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] < size or (t.shape[0] != size and not least) \
+            or t.device != device or not t.is_contiguous():
         raise KernelError(f"{what}: expected {size} contiguous fp32 values on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
@@ -104,8 +108,7 @@ def _out(out: Optional[Int8Act], n: int, k: int, device):
     if k < 1 or k > MAX_K:
         raise KernelError(f"row width {k} is outside 1 .. {MAX_K}")
     if out is None:
-        out = act_buffers(n, k, device)
-        return out, (k + 15) & ~15
+        return act_buffers(n, k, device), (k + 15) & ~15
     ld = _matrix(out.q, "out.q", (torch.int8,), n, k, device)
     _vector(out.scale, "out.scale", n, device, least=True)
     return out, ld

@@ -55,6 +55,12 @@ def stream() -> c_void_p:
     return c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def raw_stream(index: int) -> int:
+    """Current stream of device ``index`` as an integer. The call PyTorch's own compiled kernels use: 0.1 us instead of the
+    2 - 3 us of building a ``torch.cuda.Stream`` object, which counts in a chain of 5 us kernels."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 launches = 0        # kernels enqueued through this module since import (each wrapper reports its count)
 
 
