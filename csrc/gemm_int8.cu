@@ -119,11 +119,11 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   auto fail = [&](int code) { if (p.err) atomicCAS(p.err, 0, code); *abort_flag = 1; };
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       pdl_wait();
       int st = 0;
       uint32_t ph = 1;
-      for (int s = s0; s < s1 && !*abort_flag; ++s) {
+      for (int s = s0; s < s1; ++s) {
         if (!mbar_wait(empty + st, ph)) { fail(VG_ERR_EMPTY_WAIT); break; }
         uint8_t* a = smem + st * S::STAGE;
         mbar_arrive_expect_tx(full + st, S::STAGE);
@@ -133,22 +133,23 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_i8(BM, BN);
-      int st = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int s = s0; s < s1 && !*abort_flag; ++s) {
-        if (!mbar_wait(full + st, ph)) { fail(VG_ERR_TMA_WAIT); ok = false; break; }
-        tc_fence_after();
-        const uint32_t a = smem_u32(smem + st * S::STAGE), b = a + A_BYTES;
+    constexpr uint32_t idesc = idesc_i8(BM, BN);
+    const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), bdesc0 = umma_desc_sw128(smem_u32(smem) + A_BYTES);
+    int st = 0;
+    uint32_t ph = 0;
+    for (int s = s0; s < s1; ++s) {
+      if (!mbar_wait(full + st, ph)) { fail(VG_ERR_TMA_WAIT); break; }
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t off = (uint64_t)(st * (S::STAGE >> 4));
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk)
-          umma_i8(tmem, umma_desc_sw128(a + kk * 32), umma_desc_sw128(b + kk * 32), idesc, (s > s0 || kk) ? 1u : 0u);
+          umma_i8(tmem, adesc0 + off + kk * 2, bdesc0 + off + kk * 2, idesc, (s > s0 || kk) ? 1u : 0u);
         umma_commit(empty + st);
-        if (++st == S::STAGES) { st = 0; ph ^= 1; }
+        if (s == s1 - 1) umma_commit(acc_full);
       }
-      if (ok && s1 > s0) umma_commit(acc_full);
+      __syncwarp();
+      if (++st == S::STAGES) { st = 0; ph ^= 1; }
     }
   } else {
     pdl_wait();
@@ -160,7 +161,7 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
   const int cols = min(BN, p.N - n0);                      // columns that hold a token
   bool have = false;
-  if (warp >= 2 && s1 > s0 && __all_sync(0xffffffffu, !*abort_flag)) {
+  if (warp >= 2 && s1 > s0) {
     have = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));
     if (!have) fail(VG_ERR_MMA_WAIT);
     tc_fence_after();
@@ -326,7 +327,7 @@ gemm_int8_pair_kernel(const I8Params p, const int bn, const PairTiles tiles, con
   auto fail = [&](int code) { if (p.err) atomicCAS(p.err, 0, code); *abort_flag = 1; };
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       pdl_wait();
       const uint32_t tx = 2 * (uint32_t)(A_BYTES + bn / 2 * BK);
       const uint32_t full0 = dsmem_map(smem_u32(full), 0);
@@ -338,7 +339,7 @@ gemm_int8_pair_kernel(const I8Params p, const int bn, const PairTiles tiles, con
         tiles.at(t, mi, ni);
         const int m0 = mi * 2 * BM + rank * BM, n0 = ni * bn + rank * (bn / 2);
         for (int s = 0; s < slabs; ++s) {
-          if (*abort_flag || !mbar_wait(empty + st, ph)) { if (!*abort_flag) fail(VG_ERR_EMPTY_WAIT); ok = false; break; }
+          if (!mbar_wait(empty + st, ph)) { fail(VG_ERR_EMPTY_WAIT); ok = false; break; }
           const uint32_t a = smem_u32(smem + st * P_STAGE), bar = full0 + st * 8;
           if (rank == 0) mbar_arrive_expect_tx(full + st, tx);
           tma_pair_g2s(a, &tm_w, s * BK, m0, bar);
@@ -355,8 +356,11 @@ gemm_int8_pair_kernel(const I8Params p, const int bn, const PairTiles tiles, con
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    // The whole warp walks the loop and one elected lane issues: descriptors then stay in uniform registers. (With the
+    // loop inside a lane == 0 branch each MMA took 70 cycles to issue and a slab 330 more: 0.35 us a slab at any width.)
+    if (rank == 0) {
       const uint32_t idesc = idesc_i8(2 * BM, bn);
+      const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), bdesc0 = umma_desc_sw128(smem_u32(smem) + A_BYTES);
       int st = 0, it = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -364,17 +368,21 @@ gemm_int8_pair_kernel(const I8Params p, const int bn, const PairTiles tiles, con
         const int buf = it & 1;
         if (!mbar_wait(acc_empty + buf, ((it >> 1) & 1) ^ 1)) { fail(VG_ERR_MMA_WAIT); break; }
         tc_fence_after();
+        const uint32_t acc = tmem + buf * PBN;
         for (int s = 0; s < slabs; ++s) {
-          if (*abort_flag || !mbar_wait(full + st, ph)) { if (!*abort_flag) fail(VG_ERR_TMA_WAIT); ok = false; break; }
+          if (!mbar_wait(full + st, ph)) { fail(VG_ERR_TMA_WAIT); ok = false; break; }
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + st * P_STAGE), b = a + A_BYTES;
+          if (elect_one()) {
+            const uint64_t off = (uint64_t)(st * (P_STAGE >> 4));
 #pragma unroll
-          for (int kk = 0; kk < BK / 32; ++kk)
-            umma_i8_pair(tmem + buf * PBN, umma_desc_sw128(a + kk * 32), umma_desc_sw128(b + kk * 32), idesc, (s || kk) ? 1u : 0u);
-          umma_commit_pair(empty + st);
+            for (int kk = 0; kk < BK / 32; ++kk)
+              umma_i8_pair(acc, adesc0 + off + kk * 2, bdesc0 + off + kk * 2, idesc, (s || kk) ? 1u : 0u);
+            umma_commit_pair(empty + st);
+            if (s == slabs - 1) umma_commit_pair(acc_full + buf);
+          }
+          __syncwarp();
           if (++st == P_STAGES) { st = 0; ph ^= 1; }
         }
-        if (ok) umma_commit_pair(acc_full + buf);
       }
     }
   } else {
@@ -394,8 +402,7 @@ gemm_int8_pair_kernel(const I8Params p, const int bn, const PairTiles tiles, con
       for (int c = lane; c < cols; c += 32) sx[c] = __ldg(p.sx + n0 + c);
       const float sw = m < p.M ? __ldg(p.sw + m) : 0.f;
       __syncwarp();
-      const bool got = !*abort_flag && mbar_wait(acc_full + buf, (it >> 1) & 1);
-      if (!__all_sync(0xffffffffu, got)) { if (!*abort_flag) fail(VG_ERR_MMA_WAIT); break; }
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full + buf, (it >> 1) & 1))) { fail(VG_ERR_MMA_WAIT); break; }
       tc_fence_after();
       const uint32_t acc = tmem + buf * PBN + ((uint32_t)(quarter * 32) << 16);
       for (int c = 0; c < cols; c += 32) {
