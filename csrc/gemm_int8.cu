@@ -1,17 +1,18 @@
 // Integer matrix product of the W8A8 path on the 5th-generation tensor cores (tcgen05.mma kind::i8).
 //
-//   out[n, m] = (sum_k q[n, k] * c[m, k]) * sx[n] * sw[m]
+//   out[n, m] = (sum_k q[n, k] * c[m, k]) * sw[m] * sx[n]
 //
 // q: int8 tokens with a scale each, c: int8 weights with a scale per output channel, both row-major as the quantisers
 // write them. The sum is exact: int32 accumulators cannot overflow for K <= 131071 (128 * 128 * K < 2^31), so neither
 // the tile shape nor the split of K shows in the result and a token's bits do not depend on the batch.
 //
-// Weights are the A operand (128 output channels = the 128 TMEM lanes), BN tokens the B operand. Slabs of 128 bytes of
-// K of both arrive by tiled TMA with the 128-byte swizzle (zeros beyond K, the channels and the tokens).
-// CTA (192 threads): warp 0 copies, warp 1 issues four K = 32 MMAs per slab, warps 2-5 read the accumulator back,
-// thread = output channel, so a warp stores 32 neighbouring channels of one token. With few tiles K is split over a
-// cluster: every CTA sends the columns of its partial sums to the CTA that owns them (distributed shared memory).
-// All waits are bounded.
+// Weights are the A operand (output channels = the 128 TMEM lanes of a CTA), tokens the B operand. Slabs of 128 bytes of
+// K of both arrive by tiled TMA with the 128-byte swizzle (zeros beyond K, the channels and the tokens). Two forms:
+//   narrow  up to 64 tokens: one CTA per 128 channels, bound by the weight stream
+//   pair    more: a pair of CTAs per 256 channels x up to 256 tokens (cta_group::2), bound by the MMAs
+// Both have 192 threads: warp 0 copies, warp 1 issues four K = 32 MMAs per slab, warps 2-5 read the accumulator back,
+// thread = output channel. With few tiles K is split over a cluster and the partial sums meet in distributed shared
+// memory. All waits are bounded.
 #include <cuda.h>
 #include <atomic>
 #include <mutex>
@@ -34,6 +35,7 @@ struct I8Params {
   void* out;
   long long ldo;
   int M, N, K, split, out_f32;
+  int vec;                                  // four channels of a token can be stored at once
   int* err;
 };
 
@@ -49,37 +51,142 @@ VG_DEVINL void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-VG_DEVINL void dsmem_st_s32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+VG_DEVINL void dsmem_st_v4(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+// L2 only: safe before the wait for the predecessor kernel, which may still be writing these bytes (L2 is where its
+// stores and the later loads meet)
+VG_DEVINL void tma_prefetch_l2(const void* tmap, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tmap), "r"(c0), "r"(c1) : "memory");
+}
+VG_DEVINL void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
 }
 
+// Where a warp's stores go: 32 channels (this lane's is `m`) of the tokens from n0 on.
+struct OutWarp {
+  char* base;               // vec: token (lane & 3), the first of the four channels around this lane; else token 0, channel m
+  size_t pitch;             // bytes between tokens
+  float sw;
+  bool in;                  // this lane has something to store
+  VG_DEVINL OutWarp(const I8Params& p, int m, int n0) {
+    const int lane = threadIdx.x & 31, es = p.out_f32 ? 4 : 2;
+    pitch = (size_t)p.ldo * es;
+    sw = m < p.M ? __ldg(p.sw + m) : 0.f;
+    in = m < p.M;           // vec needs M % 4 == 0: the four channels are inside or outside together
+    base = static_cast<char*>(p.out) + (p.vec ? (size_t)(n0 + (lane & 3)) * pitch + (size_t)(m & ~3) * es
+                                              : (size_t)n0 * pitch + (size_t)m * es);
+  }
+};
+
+// Stores columns [c, c + 4) (`v`, int32 sums of this lane's channel), `left` of which hold a token. A warp has 32
+// channels of one token per register, so storing registers as they are takes one 2-byte store per value and lane: 50
+// cycles a column, 13 k cycles for a 256-column tile against 20 k of MMAs at K = 5120. The vec form transposes 4 x 4
+// blocks among neighbouring lanes first (two shuffles), then each lane stores four channels of one token.
+VG_DEVINL void store4(const I8Params& p, const OutWarp& o, int c, const uint32_t* v, const float4 sx, int left) {
+  const float y0 = (float)(int)v[0] * o.sw * sx.x, y1 = (float)(int)v[1] * o.sw * sx.y;
+  const float y2 = (float)(int)v[2] * o.sw * sx.z, y3 = (float)(int)v[3] * o.sw * sx.w;
+  if (!p.vec) {
+    const float y[4] = {y0, y1, y2, y3};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (o.in && i < left) {
+        char* d = o.base + (size_t)(c + i) * o.pitch;
+        if (p.out_f32) *reinterpret_cast<float*>(d) = y[i];
+        else *reinterpret_cast<__nv_bfloat16*>(d) = __float2bfloat16_rn(y[i]);
+      }
+    }
+    return;
+  }
+  const bool b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
+  char* d = o.base + (size_t)c * o.pitch;
+  const bool st = o.in && (int)(threadIdx.x & 3) < left;
+  if (p.out_f32) {
+    const float ra = __shfl_xor_sync(0xffffffffu, b0 ? y0 : y1, 1), rb = __shfl_xor_sync(0xffffffffu, b0 ? y2 : y3, 1);
+    const float2 A = b0 ? make_float2(ra, y1) : make_float2(y0, ra);      // token b0, channels (even, odd)
+    const float2 B = b0 ? make_float2(rb, y3) : make_float2(y2, rb);      // token 2 + b0
+    const float2 snd = b1 ? A : B, own = b1 ? B : A;
+    const float2 rcv = make_float2(__shfl_xor_sync(0xffffffffu, snd.x, 2), __shfl_xor_sync(0xffffffffu, snd.y, 2));
+    if (st) *reinterpret_cast<float4*>(d) = b1 ? make_float4(rcv.x, rcv.y, own.x, own.y) : make_float4(own.x, own.y, rcv.x, rcv.y);
+  } else {
+    const __nv_bfloat162 e2 = __floats2bfloat162_rn(y0, y2), o2 = __floats2bfloat162_rn(y1, y3);
+    const uint32_t e = *reinterpret_cast<const uint32_t*>(&e2), q = *reinterpret_cast<const uint32_t*>(&o2);
+    const uint32_t own = b0 ? q : e, rcv = __shfl_xor_sync(0xffffffffu, b0 ? e : q, 1);
+    const uint32_t lo = b0 ? rcv : own, hi = b0 ? own : rcv;              // even channel, odd channel
+    const uint32_t w0 = __byte_perm(lo, hi, 0x5410), w1 = __byte_perm(lo, hi, 0x7632);   // tokens b0 and 2 + b0
+    const uint32_t mine = b1 ? w1 : w0, other = __shfl_xor_sync(0xffffffffu, b1 ? w0 : w1, 2);
+    if (st) *reinterpret_cast<uint2*>(d) = b1 ? make_uint2(other, mine) : make_uint2(mine, other);
+  }
+}
+// A warp's own copy of the token scales, fetched while the accumulator is still being built.
+VG_DEVINL void fetch_sx(const I8Params& p, float* sx, int n0, int cols) {
+  __syncwarp();
+  for (int c = threadIdx.x & 31; c < (cols + 31) / 32 * 32; c += 32) sx[c] = c < cols ? __ldg(p.sx + n0 + c) : 0.f;
+  __syncwarp();
+}
+
+// Split K: columns go in groups of four, group g to the part g % parts. A part's receive area (over the drained ring)
+// holds [source part][own group][channel] as 16-byte words.
+VG_DEVINL uint32_t group_slots(int cols, int parts) { return (uint32_t)(((cols + 3) / 4 + parts - 1) / parts); }
+// `to_rank(part)`: cluster rank of the CTA of that part which holds the same channels
+template <typename F>
+VG_DEVINL void send_partials(uint32_t area, uint32_t acc, bool have, int cols, int part, int parts, int r, F to_rank) {
+  const uint32_t slots = group_slots(cols, parts);
+  int dst = 0;
+  uint32_t slot = 0;
+  for (int c = 0; c < cols; c += 16) {
+    uint32_t v[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    if (have) {
+      tmem_ld8(acc + c, v);
+      if (c + 8 < cols) tmem_ld8(acc + c + 8, v + 8);
+      tmem_ld_wait();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (c + 4 * i < cols) dsmem_st_v4(dsmem_map(area + ((part * slots + slot) * BM + r) * 16, to_rank(dst)), v + 4 * i);
+      if (++dst == parts) { dst = 0; ++slot; }
+    }
+  }
+}
+VG_DEVINL void finish_partials(const I8Params& p, const uint8_t* area, const OutWarp& o, const float* sx, int cols, int part, int parts,
+                               int r) {
+  const uint32_t slots = group_slots(cols, parts);
+  const uint4* a = reinterpret_cast<const uint4*>(area) + r;
+  for (uint32_t s = 0; s < slots; ++s) {
+    const int c = ((int)s * parts + part) * 4;
+    if (c >= cols) break;
+    uint32_t v[4] = {0, 0, 0, 0};
+    for (int q = 0; q < parts; ++q) {
+      const uint4 w = a[(q * slots + s) * BM];
+      v[0] += w.x; v[1] += w.y; v[2] += w.z; v[3] += w.w;
+    }
+    store4(p, o, c, v, *reinterpret_cast<const float4*>(sx + c), cols - c);
+  }
+}
+
+// ------------------------------------------------------------------ narrow form
 template <int BN>
 struct Shape {
   static constexpr int B_BYTES = BN * BK;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  // two CTAs per SM while the token tile is small (the weight stream wants many loads in flight), else one
-  static constexpr int CTAS = BN <= 64 ? 2 : 1;
-  static constexpr int STAGES = (CTAS == 2 ? 108 : 216) * 1024 / STAGE;
+  static constexpr int STAGES = 108 * 1024 / STAGE;       // two CTAs per SM: the weight stream wants many loads in flight
   static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
-  static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
+  static constexpr int SX = STAGES * STAGE + 256;         // [4 warps][BN] token scales (64 at least: fetched 32 at a time)
+  static constexpr int SMEM = SX + 4 * 64 * 4 + 1024;
   static_assert(STAGES * 16 + 32 <= 256, "barrier area");
+  static_assert((BN / 4 + MAX_SPLIT) * BM * 16 <= STAGES * STAGE, "partial sums over the ring");
 };
 
-// `v` holds columns [c0, c0 + 8) of this thread's channel.
-VG_DEVINL void store8(const I8Params& p, int m, int n0, const uint32_t* v, float sw) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int n = n0 + i;
-    if (n < p.N) {
-      const float y = (float)(int)v[i] * sw * __ldg(p.sx + n);
-      if (p.out_f32) static_cast<float*>(p.out)[(size_t)n * p.ldo + m] = y;
-      else static_cast<__nv_bfloat16*>(p.out)[(size_t)n * p.ldo + m] = __float2bfloat16_rn(y);
-    }
-  }
-}
-
 template <int BN>
-__global__ void __launch_bounds__(THREADS, Shape<BN>::CTAS)
+__global__ void __launch_bounds__(THREADS, 2)
 gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x) {
   using S = Shape<BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -120,6 +227,7 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
 
   if (warp == 0) {
     if (elect_one()) {
+      for (int s = s0; s < min(s1, s0 + S::STAGES); ++s) tma_prefetch_l2(&tm_w, s * BK, m0);
       pdl_wait();
       int st = 0;
       uint32_t ph = 1;
@@ -160,58 +268,30 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   const int r = quarter * 32 + lane;                       // channel row of this thread within the tile
   const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
   const int cols = min(BN, p.N - n0);                      // columns that hold a token
+  float* sx = reinterpret_cast<float*>(smem + S::SX) + quarter * 64;
   bool have = false;
-  if (warp >= 2 && s1 > s0) {
+  if (warp >= 2) {
+    fetch_sx(p, sx, n0, cols);
     have = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));
     if (!have) fail(VG_ERR_MMA_WAIT);
     tc_fence_after();
   }
   if (p.split == 1) {
     if (have) {
-      const int m = m0 + r;
-      const float sw = m < p.M ? p.sw[m] : 0.f;
+      const OutWarp o(p, m0 + r, n0);
       for (int c = 0; c < cols; c += 8) {
         uint32_t v[8];
         tmem_ld8(lane_base + c, v);
         tmem_ld_wait();
-        if (m < p.M) store8(p, m, n0 + c, v, sw);
+        store4(p, o, c, v, *reinterpret_cast<const float4*>(sx + c), cols - c);
+        if (c + 4 < cols) store4(p, o, c + 4, v + 4, *reinterpret_cast<const float4*>(sx + c + 4), cols - c - 4);
       }
     }
   } else {
-    // columns [rank * own, ...) of the tile belong to cluster rank `rank`; its receive area (over the drained ring)
-    // holds [source rank][column][channel]
-    const int own = (BN + p.split - 1) / p.split;
     cluster_sync_all();                                    // every CTA's MMAs are done: the rings are free
-    if (warp >= 2) {
-      const uint32_t area = smem_u32(smem);
-      for (int c = 0; c < cols; c += 8) {
-        uint32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (have) {
-          tmem_ld8(lane_base + c, v);
-          tmem_ld_wait();
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c + i < cols)
-            dsmem_st_s32(dsmem_map(area + (uint32_t)(((rank * own + (c + i) % own) * BM + r) * 4), (c + i) / own), v[i]);
-      }
-    }
+    if (warp >= 2) send_partials(smem_u32(smem), lane_base, have, cols, rank, p.split, r, [](int q) { return (uint32_t)q; });
     cluster_sync_all();
-    if (warp >= 2) {
-      const int m = m0 + r;
-      const float sw = m < p.M ? p.sw[m] : 0.f;
-      const int* area = reinterpret_cast<const int*>(smem);
-      const int c1 = min(cols, (rank + 1) * own);
-      for (int c = rank * own; c < c1; ++c) {
-        int sum = 0;
-        for (int q = 0; q < p.split; ++q) sum += area[(q * own + c - rank * own) * BM + r];
-        if (m < p.M) {
-          const float y = (float)sum * sw * __ldg(p.sx + n0 + c);
-          if (p.out_f32) static_cast<float*>(p.out)[(size_t)(n0 + c) * p.ldo + m] = y;
-          else static_cast<__nv_bfloat16*>(p.out)[(size_t)(n0 + c) * p.ldo + m] = __float2bfloat16_rn(y);
-        }
-      }
-    }
+    if (warp >= 2) finish_partials(p, smem, OutWarp(p, m0 + r, n0), sx, cols, rank, p.split, r);
   }
   if (*abort_flag && threadIdx.x == 0) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);       // let copies in flight land before the block ends
@@ -221,20 +301,24 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   if (warp == 1) tmem_dealloc(tmem, S::TMEM_COLS);
 }
 
-// ------------------------------------------------------------------ wide form: CTA pairs
-// Enough tokens to keep the tensor cores busy: a pair of CTAs (cta_group::2) owns 256 channels x BN tokens, each CTA
-// loads its 128 channels and half of the tokens, so a byte of either operand that comes from L2 feeds twice the MMA work
-// of a single-CTA tile (the 16 KB + BN * 64 B that a CTA fetches per slab is what bounds this kernel, not the MMAs).
-// Persistent: one pair per two SMs walks the tiles with two accumulators in TMEM, so a tile's stores run under the next
-// tile's MMAs. Tiles go token-first within groups of PAIR_GROUP token tiles: the weights of the running tiles and the
-// group's tokens stay in L2.
+// ------------------------------------------------------------------ pair form
+// A pair of CTAs owns 256 channels x BN tokens; each loads its 128 channels and half of the tokens, so a byte of either
+// operand that comes from L2 feeds twice the MMA work of a single-CTA tile. A slab takes 2 cycles per token of the tile
+// (512 cycles at 256: the nominal rate of the tensor cores, seen with clock stamps), and copies keep up from 128 tokens on.
+// Whole K: persistent, one pair per two SMs walks the tiles with two accumulators in TMEM, so a tile's stores run under
+// the next tile's MMAs. Tiles go token-first within groups of PAIR_GROUP token tiles: the weights of the running tiles and
+// the group's tokens stay in L2.
+// Split K: a cluster of `split` pairs per tile, one tile per cluster.
 constexpr int PBN = 256;                                  // token tile at most; BN is any multiple of 32 up to it
-constexpr int P_STAGE = A_BYTES + PBN / 2 * BK;           // 32 KB
-constexpr int P_STAGES = 6;
-constexpr int P_SX = P_STAGES * P_STAGE;                  // [4 warps][PBN] token scales
+constexpr int P_RING = 192 * 1024;                        // stages of 16 KB + 64 * BN bytes
+constexpr int P_MAX_STAGES = 10;
+constexpr int P_SX = P_RING;                              // [4 warps][PBN] token scales
 constexpr int P_BARS = P_SX + 4 * PBN * 4;
 constexpr int P_SMEM = P_BARS + 256 + 1024;
 constexpr int PAIR_GROUP = 16;
+constexpr int PAIR_MAX_SPLIT = 4;
+static_assert((PBN / 4 + PAIR_MAX_SPLIT) * BM * 16 <= P_RING, "partial sums over the ring");
+static_assert(P_MAX_STAGES * 16 + 48 <= 256, "barrier area");
 
 VG_DEVINL void tma_pair_g2s(uint32_t dst, const void* tmap, int c0, int c1, uint32_t bar) {
   asm volatile(
@@ -251,27 +335,15 @@ VG_DEVINL void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uin
       : "memory");
 }
 // arrives on the barrier at this offset in both CTAs of the pair once the MMAs issued so far are done
-VG_DEVINL void umma_commit_pair(uint64_t* bar) {
+VG_DEVINL void umma_commit_pair(uint64_t* bar, uint16_t pair_mask) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"(pair_mask)
       : "memory");
 }
 VG_DEVINL void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-VG_DEVINL void tmem_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-
 struct PairTiles {
   int mt, nt, total;
   VG_DEVINL void at(int t, int& m, int& n) const {
@@ -282,27 +354,37 @@ struct PairTiles {
   }
 };
 
-template <bool F32>
+struct PairShape {
+  int bn, stage, stages;                                 // token tile, bytes of a ring stage, number of them
+  PairTiles tiles;
+};
+
+template <bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm_int8_pair_kernel(const I8Params p, const int bn, const PairTiles tiles, const __grid_constant__ CUtensorMap tm_w,
+gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constant__ CUtensorMap tm_w,
                       const __grid_constant__ CUtensorMap tm_x) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + P_BARS);      // the leader's counts both CTAs' copies
-  uint64_t* empty = full + P_STAGES;
-  uint64_t* acc_full = empty + P_STAGES;                             // [2]
+  uint64_t* empty = full + P_MAX_STAGES;
+  uint64_t* acc_full = empty + P_MAX_STAGES;                         // [2]
   uint64_t* acc_empty = acc_full + 2;                                // [2], the leader's counts both CTAs' epilogue warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_ctarank();
-  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const int crank = (int)cluster_ctarank();
+  const int rank = crank & 1, leader = crank & ~1;                   // within the pair / the pair's first CTA
+  const int part = SPLIT ? crank >> 1 : 0;
+  const int first = SPLIT ? (int)blockIdx.x / (2 * p.split) : (int)blockIdx.x >> 1;
+  const int step = SPLIT ? sh.tiles.total : (int)gridDim.x >> 1;     // split: one tile per cluster
   const int slabs = (p.K + BK - 1) / BK;
+  const int s0 = SPLIT ? (int)((long long)slabs * part / p.split) : 0;
+  const int s1 = SPLIT ? (int)((long long)slabs * (part + 1) / p.split) : slabs;
   pdl_trigger();
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < P_STAGES; ++i) {
+    for (int i = 0; i < sh.stages; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
     }
@@ -326,101 +408,95 @@ gemm_int8_pair_kernel(const I8Params p, const int bn, const PairTiles tiles, con
   const uint32_t tmem = *tmem_slot;
   auto fail = [&](int code) { if (p.err) atomicCAS(p.err, 0, code); *abort_flag = 1; };
 
+  const int quarter = warp & 3;
+  const int r = quarter * 32 + lane;                                 // channel of this thread within the CTA's 128
+  float* sx = reinterpret_cast<float*>(smem + P_SX) + quarter * PBN;
+  bool have = false;
   if (warp == 0) {
     if (elect_one()) {
+      int mi, ni;
+      sh.tiles.at(first, mi, ni);
+      for (int s = s0; s < min(s1, s0 + sh.stages); ++s) tma_prefetch_l2(&tm_w, s * BK, mi * 2 * BM + rank * BM);
       pdl_wait();
-      const uint32_t tx = 2 * (uint32_t)(A_BYTES + bn / 2 * BK);
-      const uint32_t full0 = dsmem_map(smem_u32(full), 0);
+      const uint32_t tx = 2 * (uint32_t)sh.stage;
+      const uint32_t full0 = dsmem_map(smem_u32(full), leader);
       int st = 0, issued = 0;
       uint32_t ph = 1;
       bool ok = true;
-      for (int t = pair; t < tiles.total && ok; t += npairs) {
-        int mi, ni;
-        tiles.at(t, mi, ni);
-        const int m0 = mi * 2 * BM + rank * BM, n0 = ni * bn + rank * (bn / 2);
-        for (int s = 0; s < slabs; ++s) {
+      for (int t = first; t < sh.tiles.total && ok; t += step) {
+        sh.tiles.at(t, mi, ni);
+        const int m0 = mi * 2 * BM + rank * BM, n0 = ni * sh.bn + rank * (sh.bn / 2);
+        for (int s = s0; s < s1; ++s) {
           if (!mbar_wait(empty + st, ph)) { fail(VG_ERR_EMPTY_WAIT); ok = false; break; }
-          const uint32_t a = smem_u32(smem + st * P_STAGE), bar = full0 + st * 8;
+          const uint32_t a = smem_u32(smem) + st * sh.stage, bar = full0 + st * 8;
           if (rank == 0) mbar_arrive_expect_tx(full + st, tx);
           tma_pair_g2s(a, &tm_w, s * BK, m0, bar);
           tma_pair_g2s(a + A_BYTES, &tm_x, s * BK, n0, bar);
           ++issued;
-          if (++st == P_STAGES) { st = 0; ph ^= 1; }
+          if (++st == sh.stages) { st = 0; ph ^= 1; }
         }
       }
       // the pair's last commits have arrived here before this CTA may end
-      for (int i = 0; i < min(issued, P_STAGES) && ok; ++i) {
-        if (issued < P_STAGES) { st = i; ph = 0; }
+      if (issued < sh.stages) { st = 0; ph = 0; }
+      for (int i = 0; i < min(issued, sh.stages) && ok; ++i) {
         if (!mbar_wait(empty + st, ph)) { fail(VG_ERR_EMPTY_WAIT); ok = false; }
-        if (issued >= P_STAGES && ++st == P_STAGES) { st = 0; ph ^= 1; }
+        if (++st == sh.stages) { st = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
     // The whole warp walks the loop and one elected lane issues: descriptors then stay in uniform registers. (With the
     // loop inside a lane == 0 branch each MMA took 70 cycles to issue and a slab 330 more: 0.35 us a slab at any width.)
     if (rank == 0) {
-      const uint32_t idesc = idesc_i8(2 * BM, bn);
+      const uint32_t idesc = idesc_i8(2 * BM, sh.bn);
+      const uint16_t mask = (uint16_t)(3u << leader);
       const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), bdesc0 = umma_desc_sw128(smem_u32(smem) + A_BYTES);
       int st = 0, it = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int t = pair; t < tiles.total && ok; t += npairs, ++it) {
+      for (int t = first; t < sh.tiles.total && ok; t += step, ++it) {
         const int buf = it & 1;
         if (!mbar_wait(acc_empty + buf, ((it >> 1) & 1) ^ 1)) { fail(VG_ERR_MMA_WAIT); break; }
         tc_fence_after();
         const uint32_t acc = tmem + buf * PBN;
-        for (int s = 0; s < slabs; ++s) {
+        for (int s = s0; s < s1; ++s) {
           if (!mbar_wait(full + st, ph)) { fail(VG_ERR_TMA_WAIT); ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t off = (uint64_t)(st * (P_STAGE >> 4));
+            const uint64_t off = (uint64_t)(st * (sh.stage >> 4));
 #pragma unroll
             for (int kk = 0; kk < BK / 32; ++kk)
-              umma_i8_pair(acc, adesc0 + off + kk * 2, bdesc0 + off + kk * 2, idesc, (s || kk) ? 1u : 0u);
-            umma_commit_pair(empty + st);
-            if (s == slabs - 1) umma_commit_pair(acc_full + buf);
+              umma_i8_pair(acc, adesc0 + off + kk * 2, bdesc0 + off + kk * 2, idesc, (s > s0 || kk) ? 1u : 0u);
+            umma_commit_pair(empty + st, mask);
+            if (s == s1 - 1) umma_commit_pair(acc_full + buf, mask);
           }
           __syncwarp();
-          if (++st == P_STAGES) { st = 0; ph ^= 1; }
+          if (++st == sh.stages) { st = 0; ph ^= 1; }
         }
       }
     }
   } else {
     pdl_wait();
-    const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;
-    float* sx = reinterpret_cast<float*>(smem + P_SX) + quarter * PBN;
-    const uint32_t acc_empty0 = dsmem_map(smem_u32(acc_empty), 0);
+    const uint32_t acc_empty0 = dsmem_map(smem_u32(acc_empty), leader);
     int it = 0;
-    for (int t = pair; t < tiles.total; t += npairs, ++it) {
+    for (int t = first; t < sh.tiles.total; t += step, ++it) {
       const int buf = it & 1;
       int mi, ni;
-      tiles.at(t, mi, ni);
-      const int m = mi * 2 * BM + rank * BM + r, n0 = ni * bn;
-      const int cols = min(bn, p.N - n0);
-      __syncwarp();
-      for (int c = lane; c < cols; c += 32) sx[c] = __ldg(p.sx + n0 + c);
-      const float sw = m < p.M ? __ldg(p.sw + m) : 0.f;
-      __syncwarp();
-      if (!__all_sync(0xffffffffu, mbar_wait(acc_full + buf, (it >> 1) & 1))) { fail(VG_ERR_MMA_WAIT); break; }
+      sh.tiles.at(t, mi, ni);
+      const int n0 = ni * sh.bn, cols = min(sh.bn, p.N - n0);
+      fetch_sx(p, sx, n0, cols);
+      const OutWarp o(p, mi * 2 * BM + rank * BM + r, n0);
+      have = __all_sync(0xffffffffu, mbar_wait(acc_full + buf, (it >> 1) & 1));
+      if (!have) { fail(VG_ERR_MMA_WAIT); break; }
       tc_fence_after();
+      if (SPLIT) break;
       const uint32_t acc = tmem + buf * PBN + ((uint32_t)(quarter * 32) << 16);
       for (int c = 0; c < cols; c += 32) {
         uint32_t v[32];
         tmem_ld32(acc + c, v);
         tmem_ld_wait();
-        if (m < p.M) {
-          char* o = static_cast<char*>(p.out) + ((size_t)(n0 + c) * p.ldo + m) * (F32 ? 4 : 2);
-          const size_t step = (size_t)p.ldo * (F32 ? 4 : 2);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (c + i < cols) {
-              const float y = (float)(int)v[i] * sw * sx[c + i];
-              if (F32) *reinterpret_cast<float*>(o + i * step) = y;
-              else *reinterpret_cast<__nv_bfloat16*>(o + i * step) = __float2bfloat16_rn(y);
-            }
-          }
-        }
+        for (int i = 0; i < 32; i += 4)
+          if (c + i < cols) store4(p, o, c + i, v + i, *reinterpret_cast<const float4*>(sx + c + i), cols - c - i);
       }
       tc_fence_before();
       __syncwarp();
@@ -428,10 +504,22 @@ gemm_int8_pair_kernel(const I8Params p, const int bn, const PairTiles tiles, con
     }
   }
   __syncwarp();
+  if (SPLIT) {
+    int mi, ni;
+    sh.tiles.at(first, mi, ni);
+    const int n0 = ni * sh.bn, cols = min(sh.bn, p.N - n0);
+    cluster_sync_all();                                              // every CTA's MMAs are done: the rings are free
+    if (warp >= 2)
+      send_partials(smem_u32(smem), tmem + ((uint32_t)(quarter * 32) << 16), have, cols, part, p.split, r,
+                    [rank](int q) { return (uint32_t)(2 * q + rank); });
+    cluster_sync_all();
+    if (warp >= 2) finish_partials(p, smem, OutWarp(p, mi * 2 * BM + rank * BM + r, n0), sx, cols, part, p.split, r);
+  }
   if (*abort_flag && threadIdx.x == 0) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);       // let copies in flight land before the block ends
   }
   tc_fence_before();
+  __syncwarp();
   cluster_sync_all();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
@@ -465,15 +553,11 @@ int make_map(const void* base, int rows, int k, long long ld, int box_rows, CUte
   return r == CUDA_SUCCESS ? 0 : -(int)r - 100;
 }
 
-int sm_count(int dev) {
-  static std::atomic<int> known[64];
-  int n = known[dev & 63].load();
-  if (n <= 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    known[dev & 63].store(n);
-  }
-  return n;
-}
+// Clusters of 1 .. 8 CTAs the device holds at once with one CTA per SM (clusters stay within a GPC, so 8 CTAs leave more
+// SMs idle than 2). The runtime counts one CTA per SM for any kernel that allocates TMEM.
+struct Room {
+  int sms, clusters[MAX_SPLIT + 1];
+};
 
 // The attribute belongs to the device's copy of a kernel: set once per kernel and device.
 int allow_smem(const void* kernel, int bytes, int dev, std::atomic<unsigned long long>& done) {
@@ -484,17 +568,64 @@ int allow_smem(const void* kernel, int bytes, int dev, std::atomic<unsigned long
   return (int)e;
 }
 
-template <bool F32>
-int launch_pair(const I8Params& p, int bn, int pairs, int dev, const CUtensorMap& tw, const CUtensorMap& tx, cudaStream_t st) {
+const Room* room_of(int dev) {
+  static Room rooms[64];
+  static std::atomic<unsigned long long> known{0};
+  static std::mutex mu;
+  const unsigned long long bit = 1ull << (dev & 63);
+  Room& room = rooms[dev & 63];
+  if (known.load() & bit) return &room;
+  std::lock_guard<std::mutex> lk(mu);
+  if (known.load() & bit) return &room;
+  if (cudaDeviceGetAttribute(&room.sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return nullptr;
   static std::atomic<unsigned long long> done{0};
-  const int rc = allow_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<F32>), P_SMEM, dev, done);
+  if (allow_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<true>), P_SMEM, dev, done)) return nullptr;
+  for (int size = 1; size <= MAX_SPLIT; ++size) {
+    cudaLaunchAttribute a;
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = size;
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size * 256);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = P_SMEM;
+    cfg.attrs = &a;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&room.clusters[size], gemm_int8_pair_kernel<true>, &cfg) != cudaSuccess) return nullptr;
+  }
+  known.fetch_or(bit);
+  return &room;
+}
+
+// Token tile and K split of the pair form: the shape with the least estimated time, in cycles.
+void choose_pair(int N, int slabs, const Room& room, PairShape* sh, int* split) {
+  const int least = (N + PBN - 1) / PBN;
+  double best = 1e30;
+  for (int nt = least; nt < least + 4; ++nt) {
+    const int bn = ((N + nt - 1) / nt + 31) / 32 * 32;
+    const int used = (N + bn - 1) / bn;
+    const double slab = max(2.0 * bn, 195 + 0.76 * bn);
+    for (int s = 1; s <= PAIR_MAX_SPLIT && s <= max(1, slabs / 4); ++s) {
+      const double waves = ceil((double)sh->tiles.mt * used / max(1, room.clusters[2 * s]));
+      const double t = waves * ((slabs + s - 1) / s) * slab + (s > 1 ? waves * (4000 + 12.0 * bn) : 2000 + 12.0 * bn);
+      if (t < best) {
+        best = t;
+        sh->bn = bn;
+        sh->tiles.nt = used;
+        *split = s;
+      }
+    }
+  }
+}
+
+template <bool SPLIT>
+int launch_pair(const I8Params& p, const PairShape& sh, int sms, int dev, const CUtensorMap& tw, const CUtensorMap& tx, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  const int rc = allow_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<SPLIT>), P_SMEM, dev, done);
   if (rc) return rc;
-  PairTiles t;
-  t.mt = (p.M + 2 * BM - 1) / (2 * BM);
-  t.nt = (p.N + bn - 1) / bn;
-  t.total = t.mt * t.nt;
-  return (int)launch_pdl_cluster(gemm_int8_pair_kernel<F32>, dim3(2 * min(pairs, t.total)), dim3(THREADS), 2u, P_SMEM, st, p, bn, t,
-                                 tw, tx);
+  const int pairs = SPLIT ? sh.tiles.total * p.split : min(sms / 2, sh.tiles.total);
+  return (int)launch_pdl_cluster(gemm_int8_pair_kernel<SPLIT>, dim3(2 * pairs), dim3(THREADS), SPLIT ? 2u * p.split : 2u, P_SMEM, st, p,
+                                 sh, tw, tx);
 }
 
 template <int BN>
@@ -516,31 +647,40 @@ extern "C" int vg_gemm_int8(const void* codes, long long ldw, const float* sw, c
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
-  const int sms = sm_count(dev);
-  if (sms <= 0) return -3;
-  const int bn = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
-  const int tiles = (M + BM - 1) / BM, ntile = (N + bn - 1) / bn, slabs = (K + BK - 1) / BK;
-  if (ntile > 65535 || (long long)tiles * ntile > (1 << 28)) return -2;
+  const Room* room = room_of(dev);
+  if (!room) return -3;
   I8Params p{};
-  p.sx = sx; p.sw = sw; p.out = out; p.ldo = ldo; p.M = M; p.N = N; p.K = K; p.out_f32 = out_f32; p.err = err;
-  // one CTA per SM at most while K is split, and at least four slabs per CTA
-  p.split = max(1, min(MAX_SPLIT, min(sms / (tiles * ntile), slabs / 4)));
+  p.sx = sx; p.sw = sw; p.out = out; p.ldo = ldo; p.M = M; p.N = N; p.K = K; p.split = 1; p.out_f32 = out_f32; p.err = err;
+  const int es = out_f32 ? 4 : 2;
+  p.vec = M % 4 == 0 && (N == 1 || ldo % 4 == 0) && reinterpret_cast<uintptr_t>(out) % (4 * es) == 0;
+  const int slabs = (K + BK - 1) / BK;
   CUtensorMap tw, tx;
   int rc = make_map(codes, M, K, ldw, BM, &tw);
   if (rc) return rc;
-  if (N > 256) {
-    const int nt = (N + PBN - 1) / PBN, pbn = ((N + nt - 1) / nt + 31) / 32 * 32;
-    rc = make_map(q, N, K, ldq, pbn / 2, &tx);
+  if (N <= 64) {
+    const int bn = N <= 16 ? 16 : N <= 32 ? 32 : 64;
+    const int tiles = (M + BM - 1) / BM;
+    if (tiles > (1 << 26)) return -2;
+    // The widest split whose clusters all run at once, two CTAs per SM, with four slabs per CTA at least. 16 x 5120 x
+    // 17408 (40 tiles): 31.8 us unsplit, 20.6 / 19.5 / 17.3 with 2 / 3 / 6 parts, 23.1 with 7 (a second wave).
+    for (int s = 2; s <= MAX_SPLIT && s <= slabs / 4; ++s)
+      if (tiles <= 2 * room->clusters[s]) p.split = s;
+    rc = make_map(q, N, K, ldq, bn, &tx);
     if (rc) return rc;
-    return out_f32 ? launch_pair<true>(p, pbn, sms / 2, dev, tw, tx, st) : launch_pair<false>(p, pbn, sms / 2, dev, tw, tx, st);
+    switch (bn) {
+      case 16: return launch<16>(p, dev, tw, tx, st);
+      case 32: return launch<32>(p, dev, tw, tx, st);
+      default: return launch<64>(p, dev, tw, tx, st);
+    }
   }
-  rc = make_map(q, N, K, ldq, bn, &tx);
+  PairShape sh{};
+  sh.tiles.mt = (M + 2 * BM - 1) / (2 * BM);
+  choose_pair(N, slabs, *room, &sh, &p.split);
+  sh.stage = A_BYTES + sh.bn / 2 * BK;
+  sh.stages = min(P_MAX_STAGES, P_RING / sh.stage);
+  if ((long long)sh.tiles.mt * sh.tiles.nt > (1 << 26)) return -2;
+  sh.tiles.total = sh.tiles.mt * sh.tiles.nt;
+  rc = make_map(q, N, K, ldq, sh.bn / 2, &tx);
   if (rc) return rc;
-  switch (bn) {
-    case 16: return launch<16>(p, dev, tw, tx, st);
-    case 32: return launch<32>(p, dev, tw, tx, st);
-    case 64: return launch<64>(p, dev, tw, tx, st);
-    case 128: return launch<128>(p, dev, tw, tx, st);
-    default: return launch<256>(p, dev, tw, tx, st);
-  }
+  return p.split > 1 ? launch_pair<true>(p, sh, room->sms, dev, tw, tx, st) : launch_pair<false>(p, sh, room->sms, dev, tw, tx, st);
 }
