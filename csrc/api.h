@@ -105,8 +105,7 @@ int vg_add_rmsnorm_int8(void* res, long long ld_res, const void* delta, long lon
 int vg_dequant_int8(const void* q, long long ldq, const float* scale, void* out, long long ldo, int dtype, int n, int k,
                     cudaStream_t stream);
 int vg_gemm_int8(const void* codes, long long ldw, const float* sw, const void* q, long long ldq, const float* sx, void* out,
-                 long long ldo, int out_f32, int M, int K, int N, void* work, long long work_bytes, int* err, cudaStream_t stream);
-long long vg_gemm_int8_work_bytes(int M, int K, int N);   // scratch that call needs on the current device (0 for most shapes)
+                 long long ldo, int out_f32, int M, int K, int N, int* err, cudaStream_t stream);
 
 int vg_add_rmsnorm(void* res, const void* delta, const float* w, void* out_f16, void* out_bf16, int N, int h, float eps,
                    int plus_one, int ld_res, int ld_delta, cudaStream_t stream);

@@ -11,9 +11,8 @@
 //   narrow  up to 64 tokens: one CTA per 128 channels, bound by the weight stream
 //   pair    more: a pair of CTAs per 256 channels x up to 256 tokens (cta_group::2), bound by the MMAs
 // Both have 192 threads: warp 0 copies, warp 1 issues four K = 32 MMAs per slab, warps 2-5 read the accumulator back,
-// thread = output channel. With few tiles K is split: over a cluster whose CTAs exchange partial sums through distributed
-// shared memory (narrow), or over all pairs in even shares with the partial sums in global memory (pair). All waits are
-// bounded, and no CTA waits for another cluster.
+// thread = output channel. With few tiles K is split over a cluster and the partial sums meet in distributed shared
+// memory. All waits are bounded.
 #include <cuda.h>
 #include <atomic>
 #include <mutex>
@@ -29,7 +28,6 @@ constexpr int BK = 128;                     // bytes of K per slab
 constexpr int A_BYTES = BM * BK;
 constexpr int THREADS = 192;
 constexpr int MAX_SPLIT = 8;
-constexpr int NARROW_MAX = 64;              // tokens
 
 struct I8Params {
   const float* sx;
@@ -307,15 +305,10 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
 // A pair of CTAs owns 256 channels x BN tokens; each loads its 128 channels and half of the tokens, so a byte of either
 // operand that comes from L2 feeds twice the MMA work of a single-CTA tile. A slab takes 2 cycles per token of the tile
 // (512 cycles at 256: the nominal rate of the tensor cores, seen with clock stamps), and copies keep up from 128 tokens on.
-// Persistent: one pair per two SMs walks its share with two accumulators in TMEM, so a tile's stores run under the next
-// tile's MMAs. Tiles go token-first within groups of PAIR_GROUP token tiles: the weights of the running tiles and the
-// group's tokens stay in L2.
-//
-// Tiles rarely divide evenly among 74 pairs (40 of them at 512 x 5120 outputs leave 34 pairs idle), so the first `shared`
-// tiles are one long row of slabs that the pairs cut into equal pieces; the other tiles go whole, in turn. A pair that
-// holds only part of a tile's K writes its int32 partial sums to `work` and counts itself on the tile; the one that
-// counts last adds the others' to its own, still in TMEM, and stores the tile. Whichever pair that is, the integer sum is
-// the same. Nobody waits.
+// Whole K: persistent, one pair per two SMs walks the tiles with two accumulators in TMEM, so a tile's stores run under
+// the next tile's MMAs. Tiles go token-first within groups of PAIR_GROUP token tiles: the weights of the running tiles and
+// the group's tokens stay in L2.
+// Split K: a cluster of `split` pairs per tile, one tile per cluster.
 constexpr int PBN = 256;                                  // token tile at most; BN is any multiple of 32 up to it
 constexpr int P_RING = 192 * 1024;                        // stages of 16 KB + 64 * BN bytes
 constexpr int P_MAX_STAGES = 10;
@@ -323,7 +316,8 @@ constexpr int P_SX = P_RING;                              // [4 warps][PBN] toke
 constexpr int P_BARS = P_SX + 4 * PBN * 4;
 constexpr int P_SMEM = P_BARS + 256 + 1024;
 constexpr int PAIR_GROUP = 16;
-constexpr double CUT_FIXED = 3000, CUT_TOKEN = 24; // cycles that cutting tiles costs (see choose_pair)
+constexpr int PAIR_MAX_SPLIT = 4;
+static_assert((PBN / 4 + PAIR_MAX_SPLIT) * BM * 16 <= P_RING, "partial sums over the ring");
 static_assert(P_MAX_STAGES * 16 + 48 <= 256, "barrier area");
 
 VG_DEVINL void tma_pair_g2s(uint32_t dst, const void* tmap, int c0, int c1, uint32_t bar) {
@@ -341,79 +335,31 @@ VG_DEVINL void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uin
       : "memory");
 }
 // arrives on the barrier at this offset in both CTAs of the pair once the MMAs issued so far are done
-VG_DEVINL void umma_commit_pair(uint64_t* bar) {
+VG_DEVINL void umma_commit_pair(uint64_t* bar, uint16_t pair_mask) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"(pair_mask)
       : "memory");
 }
 VG_DEVINL void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-struct PairShape {
-  int bn, stage, stages;                                 // token tile, bytes of a ring stage, number of them
-  int mt, nt, total, shared;                             // tiles: channels, tokens, all, those cut into equal pieces
-  int slabs, pairs;
-  uint32_t* count;                                       // [shared][2 CTAs], zero at launch
-  uint4* work;                                           // [pairs][2 pieces][2 CTAs][bn / 4][128 channels]
+struct PairTiles {
+  int mt, nt, total;
   VG_DEVINL void at(int t, int& m, int& n) const {
     const int per = PAIR_GROUP * mt, g = t / per, first = g * PAIR_GROUP;
     const int width = min(PAIR_GROUP, nt - first), in = t - g * per;
     m = in / width;
     n = first + in % width;
   }
-  // The shared tiles' slabs [begin(p), begin(p + 1)) are pair p's; owner() is the inverse.
-  VG_DEVINL long long begin(int p) const { return (long long)shared * slabs * p / pairs; }
-  VG_DEVINL int owner(long long u) const { return (int)(((u + 1) * pairs - 1) / ((long long)shared * slabs)); }
-  // A pair has at most two pieces of tiles: the one it starts in the middle of and the one it does not finish.
-  VG_DEVINL uint4* piece(int p, int tile, int rank) const {
-    const int which = begin(p) > (long long)tile * slabs ? 0 : 1;
-    return work + (size_t)((p * 2 + which) * 2 + rank) * (bn / 4) * BM;
-  }
 };
 
-// One pair's share in order: its piece of the shared row, then whole tiles.
-struct PairWalk {
-  const PairShape& sh;
-  long long u, u1;
-  int next_tile, tile, s0, s1;
-  VG_DEVINL PairWalk(const PairShape& shape, int pair)
-      : sh(shape), u(shape.begin(pair)), u1(shape.begin(pair + 1)), next_tile(shape.shared + pair), tile(0), s0(0), s1(0) {}
-  VG_DEVINL bool step() {
-    if (u < u1) {
-      tile = (int)(u / sh.slabs);
-      s0 = (int)(u - (long long)tile * sh.slabs);
-      s1 = (int)min((long long)sh.slabs, s0 + (u1 - u));
-      u += s1 - s0;
-      return true;
-    }
-    tile = next_tile;
-    next_tile += sh.pairs;
-    s0 = 0;
-    s1 = sh.slabs;
-    return tile < sh.total;
-  }
+struct PairShape {
+  int bn, stage, stages;                                 // token tile, bytes of a ring stage, number of them
+  PairTiles tiles;
 };
 
-// true if it is on all 128 threads of the epilogue
-VG_DEVINL bool epilogue_all(bool v) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, 1, 128, p;\n\t"
-      "selp.b32 %0, 1, 0, q;\n\t}\n"
-      : "=r"(r) : "r"((uint32_t)v) : "memory");
-  return r != 0;
-}
-
-__global__ void zero_words_kernel(uint32_t* p, int n) {
-  pdl_trigger();
-  pdl_wait();
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < n) p[i] = 0;
-}
-
+template <bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constant__ CUtensorMap tm_w,
                       const __grid_constant__ CUtensorMap tm_x) {
@@ -425,11 +371,16 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   uint64_t* acc_empty = acc_full + 2;                                // [2], the leader's counts both CTAs' epilogue warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile uint32_t* counted = tmem_slot + 2;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_ctarank();
-  const int pair = blockIdx.x >> 1;
+  const int crank = (int)cluster_ctarank();
+  const int rank = crank & 1, leader = crank & ~1;                   // within the pair / the pair's first CTA
+  const int part = SPLIT ? crank >> 1 : 0;
+  const int first = SPLIT ? (int)blockIdx.x / (2 * p.split) : (int)blockIdx.x >> 1;
+  const int step = SPLIT ? sh.tiles.total : (int)gridDim.x >> 1;     // split: one tile per cluster
+  const int slabs = (p.K + BK - 1) / BK;
+  const int s0 = SPLIT ? (int)((long long)slabs * part / p.split) : 0;
+  const int s1 = SPLIT ? (int)((long long)slabs * (part + 1) / p.split) : slabs;
   pdl_trigger();
 
   if (threadIdx.x == 0) {
@@ -457,26 +408,25 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   const uint32_t tmem = *tmem_slot;
   auto fail = [&](int code) { if (p.err) atomicCAS(p.err, 0, code); *abort_flag = 1; };
 
-  PairWalk walk(sh, pair);
+  const int quarter = warp & 3;
+  const int r = quarter * 32 + lane;                                 // channel of this thread within the CTA's 128
+  float* sx = reinterpret_cast<float*>(smem + P_SX) + quarter * PBN;
+  bool have = false;
   if (warp == 0) {
     if (elect_one()) {
-      PairWalk ahead = walk;
-      if (ahead.step()) {
-        int mi, ni;
-        sh.at(ahead.tile, mi, ni);
-        for (int s = ahead.s0; s < min(ahead.s1, ahead.s0 + sh.stages); ++s) tma_prefetch_l2(&tm_w, s * BK, mi * 2 * BM + rank * BM);
-      }
+      int mi, ni;
+      sh.tiles.at(first, mi, ni);
+      for (int s = s0; s < min(s1, s0 + sh.stages); ++s) tma_prefetch_l2(&tm_w, s * BK, mi * 2 * BM + rank * BM);
       pdl_wait();
       const uint32_t tx = 2 * (uint32_t)sh.stage;
-      const uint32_t full0 = dsmem_map(smem_u32(full), 0);
+      const uint32_t full0 = dsmem_map(smem_u32(full), leader);
       int st = 0, issued = 0;
       uint32_t ph = 1;
       bool ok = true;
-      while (ok && walk.step()) {
-        int mi, ni;
-        sh.at(walk.tile, mi, ni);
+      for (int t = first; t < sh.tiles.total && ok; t += step) {
+        sh.tiles.at(t, mi, ni);
         const int m0 = mi * 2 * BM + rank * BM, n0 = ni * sh.bn + rank * (sh.bn / 2);
-        for (int s = walk.s0; s < walk.s1; ++s) {
+        for (int s = s0; s < s1; ++s) {
           if (!mbar_wait(empty + st, ph)) { fail(VG_ERR_EMPTY_WAIT); ok = false; break; }
           const uint32_t a = smem_u32(smem) + st * sh.stage, bar = full0 + st * 8;
           if (rank == 0) mbar_arrive_expect_tx(full + st, tx);
@@ -498,25 +448,26 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
     // loop inside a lane == 0 branch each MMA took 70 cycles to issue and a slab 330 more: 0.35 us a slab at any width.)
     if (rank == 0) {
       const uint32_t idesc = idesc_i8(2 * BM, sh.bn);
+      const uint16_t mask = (uint16_t)(3u << leader);
       const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), bdesc0 = umma_desc_sw128(smem_u32(smem) + A_BYTES);
-      int st = 0;
+      int st = 0, it = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int it = 0; ok && walk.step(); ++it) {
+      for (int t = first; t < sh.tiles.total && ok; t += step, ++it) {
         const int buf = it & 1;
         if (!mbar_wait(acc_empty + buf, ((it >> 1) & 1) ^ 1)) { fail(VG_ERR_MMA_WAIT); break; }
         tc_fence_after();
         const uint32_t acc = tmem + buf * PBN;
-        for (int s = walk.s0; s < walk.s1; ++s) {
+        for (int s = s0; s < s1; ++s) {
           if (!mbar_wait(full + st, ph)) { fail(VG_ERR_TMA_WAIT); ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
             const uint64_t off = (uint64_t)(st * (sh.stage >> 4));
 #pragma unroll
             for (int kk = 0; kk < BK / 32; ++kk)
-              umma_i8_pair(acc, adesc0 + off + kk * 2, bdesc0 + off + kk * 2, idesc, (s > walk.s0 || kk) ? 1u : 0u);
-            umma_commit_pair(empty + st);
-            if (s == walk.s1 - 1) umma_commit_pair(acc_full + buf);
+              umma_i8_pair(acc, adesc0 + off + kk * 2, bdesc0 + off + kk * 2, idesc, (s > s0 || kk) ? 1u : 0u);
+            umma_commit_pair(empty + st, mask);
+            if (s == s1 - 1) umma_commit_pair(acc_full + buf, mask);
           }
           __syncwarp();
           if (++st == sh.stages) { st = 0; ph ^= 1; }
@@ -525,61 +476,24 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
     }
   } else {
     pdl_wait();
-    const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;                               // channel of this thread within the CTA's 128
-    float* sx = reinterpret_cast<float*>(smem + P_SX) + quarter * PBN;
-    const uint32_t acc_empty0 = dsmem_map(smem_u32(acc_empty), 0);
-    for (int it = 0; walk.step(); ++it) {
+    const uint32_t acc_empty0 = dsmem_map(smem_u32(acc_empty), leader);
+    int it = 0;
+    for (int t = first; t < sh.tiles.total; t += step, ++it) {
       const int buf = it & 1;
       int mi, ni;
-      sh.at(walk.tile, mi, ni);
+      sh.tiles.at(t, mi, ni);
       const int n0 = ni * sh.bn, cols = min(sh.bn, p.N - n0);
       fetch_sx(p, sx, n0, cols);
       const OutWarp o(p, mi * 2 * BM + rank * BM + r, n0);
-      // the four warps go on or give up together: they meet at barriers below
-      if (!epilogue_all(mbar_wait(acc_full + buf, (it >> 1) & 1))) { fail(VG_ERR_MMA_WAIT); break; }
+      have = __all_sync(0xffffffffu, mbar_wait(acc_full + buf, (it >> 1) & 1));
+      if (!have) { fail(VG_ERR_MMA_WAIT); break; }
       tc_fence_after();
+      if (SPLIT) break;
       const uint32_t acc = tmem + buf * PBN + ((uint32_t)(quarter * 32) << 16);
-      int from = 0, to = -1;                                         // the other pairs with a piece of this tile
-      bool store = true;
-      if (walk.s1 - walk.s0 < sh.slabs) {
-        const long long u = (long long)walk.tile * sh.slabs;
-        from = sh.owner(u);
-        to = sh.owner(u + sh.slabs - 1);
-        uint4* mine = sh.piece(pair, walk.tile, rank) + r;
-        for (int c = 0; c < cols; c += 32) {
-          uint32_t v[32];
-          tmem_ld32(acc + c, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            if (c + i < cols) mine[(c + i) / 4 * BM] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        }
-        __threadfence();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (threadIdx.x == 64) {
-          __threadfence();
-          *counted = atomicAdd(sh.count + walk.tile * 2 + rank, 1u);
-          __threadfence();
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        store = *counted == (uint32_t)(to - from);
-      }
-      for (int c = 0; store && c < cols; c += 32) {
+      for (int c = 0; c < cols; c += 32) {
         uint32_t v[32];
         tmem_ld32(acc + c, v);
         tmem_ld_wait();
-        for (int q = from; q <= to; ++q) {
-          if (q == pair) continue;
-          const uint4* other = sh.piece(q, walk.tile, rank) + (size_t)(c / 4) * BM + r;
-          uint4 w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = c + 4 * i < cols ? __ldcg(other + i * BM) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[4 * i] += w[i].x; v[4 * i + 1] += w[i].y; v[4 * i + 2] += w[i].z; v[4 * i + 3] += w[i].w;
-          }
-        }
 #pragma unroll
         for (int i = 0; i < 32; i += 4)
           if (c + i < cols) store4(p, o, c + i, v + i, *reinterpret_cast<const float4*>(sx + c + i), cols - c - i);
@@ -590,6 +504,17 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
     }
   }
   __syncwarp();
+  if (SPLIT) {
+    int mi, ni;
+    sh.tiles.at(first, mi, ni);
+    const int n0 = ni * sh.bn, cols = min(sh.bn, p.N - n0);
+    cluster_sync_all();                                              // every CTA's MMAs are done: the rings are free
+    if (warp >= 2)
+      send_partials(smem_u32(smem), tmem + ((uint32_t)(quarter * 32) << 16), have, cols, part, p.split, r,
+                    [rank](int q) { return (uint32_t)(2 * q + rank); });
+    cluster_sync_all();
+    if (warp >= 2) finish_partials(p, smem, OutWarp(p, mi * 2 * BM + rank * BM + r, n0), sx, cols, part, p.split, r);
+  }
   if (*abort_flag && threadIdx.x == 0) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);       // let copies in flight land before the block ends
   }
@@ -654,7 +579,7 @@ const Room* room_of(int dev) {
   if (known.load() & bit) return &room;
   if (cudaDeviceGetAttribute(&room.sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return nullptr;
   static std::atomic<unsigned long long> done{0};
-  if (allow_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel), P_SMEM, dev, done)) return nullptr;
+  if (allow_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<true>), P_SMEM, dev, done)) return nullptr;
   for (int size = 1; size <= MAX_SPLIT; ++size) {
     cudaLaunchAttribute a;
     a.id = cudaLaunchAttributeClusterDimension;
@@ -666,57 +591,41 @@ const Room* room_of(int dev) {
     cfg.dynamicSmemBytes = P_SMEM;
     cfg.attrs = &a;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&room.clusters[size], gemm_int8_pair_kernel, &cfg) != cudaSuccess) return nullptr;
+    if (cudaOccupancyMaxActiveClusters(&room.clusters[size], gemm_int8_pair_kernel<true>, &cfg) != cudaSuccess) return nullptr;
   }
   known.fetch_or(bit);
   return &room;
 }
 
-// Token tile of the pair form, and how many tiles are cut into equal pieces: the least estimated time in cycles. A slab
-// costs its MMAs (2 cycles a token) or its copies (195 cycles for the weights, 0.76 a token). Cutting adds the partial
-// sums' way through L2 and one more kernel boundary.
-void choose_pair(int N, int slabs, int mt, int sms, PairShape* sh) {
-  const int least = (N + PBN - 1) / PBN, pairs = max(1, sms / 2);
+// Token tile and K split of the pair form: the shape with the least estimated time, in cycles.
+void choose_pair(int N, int slabs, const Room& room, PairShape* sh, int* split) {
+  const int least = (N + PBN - 1) / PBN;
   double best = 1e30;
   for (int nt = least; nt < least + 4; ++nt) {
     const int bn = ((N + nt - 1) / nt + 31) / 32 * 32;
-    const long long used = (N + bn - 1) / bn, tiles = (long long)mt * used;
-    const double slab = max(2.0 * bn, 195 + 0.76 * bn), tail = 2000 + 12.0 * bn;
-    const double whole = (double)((tiles + pairs - 1) / pairs) * slabs * slab + tail;
-    const int cutters = (int)min((long long)pairs, tiles * slabs / 4);       // four slabs each at least
-    const double cut = cutters < 2 ? 1e30 : (double)tiles * slabs / cutters * slab + tail + CUT_FIXED + CUT_TOKEN * bn;
-    for (int c = 0; c < 2; ++c) {
-      if ((c ? cut : whole) >= best) continue;
-      best = c ? cut : whole;
-      sh->bn = bn;
-      sh->nt = (int)used;
-      // the remainder and one full round of tiles, so that a piece is at least half a tile
-      sh->pairs = c ? cutters : (int)min((long long)pairs, tiles);
-      const long long rest = tiles % sh->pairs, some = tiles <= 2 * sh->pairs ? tiles : sh->pairs + rest;
-      sh->shared = c ? (int)some : 0;
+    const int used = (N + bn - 1) / bn;
+    const double slab = max(2.0 * bn, 195 + 0.76 * bn);
+    for (int s = 1; s <= PAIR_MAX_SPLIT && s <= max(1, slabs / 4); ++s) {
+      const double waves = ceil((double)sh->tiles.mt * used / max(1, room.clusters[2 * s]));
+      const double t = waves * ((slabs + s - 1) / s) * slab + (s > 1 ? waves * (4000 + 12.0 * bn) : 2000 + 12.0 * bn);
+      if (t < best) {
+        best = t;
+        sh->bn = bn;
+        sh->tiles.nt = used;
+        *split = s;
+      }
     }
   }
-  sh->mt = mt;
-  sh->total = sh->mt * sh->nt;
-  sh->slabs = slabs;
-  sh->stage = A_BYTES + sh->bn / 2 * BK;
-  sh->stages = min(P_MAX_STAGES, P_RING / sh->stage);
-}
-long long pair_count_bytes(const PairShape& sh) { return ((long long)sh.shared * 2 * 4 + 1023) / 1024 * 1024; }
-long long pair_work_bytes(const PairShape& sh) {
-  return sh.shared ? pair_count_bytes(sh) + (long long)sh.pairs * 4 * sh.bn * BM * 4 : 0;
 }
 
-int launch_pair(const I8Params& p, const PairShape& sh, int dev, const CUtensorMap& tw, const CUtensorMap& tx, cudaStream_t st) {
+template <bool SPLIT>
+int launch_pair(const I8Params& p, const PairShape& sh, int sms, int dev, const CUtensorMap& tw, const CUtensorMap& tx, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  const int rc = allow_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel), P_SMEM, dev, done);
+  const int rc = allow_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<SPLIT>), P_SMEM, dev, done);
   if (rc) return rc;
-  if (sh.shared) {
-    const int n = sh.shared * 2;
-    const cudaError_t e = launch_pdl(zero_words_kernel, dim3((n + 255) / 256), dim3(256), 0, st, sh.count, n);
-    if (e != cudaSuccess) return (int)e;
-  }
-  return (int)launch_pdl_cluster(gemm_int8_pair_kernel, dim3(2 * sh.pairs), dim3(THREADS), 2u, P_SMEM, st, p, sh, tw, tx);
+  const int pairs = SPLIT ? sh.tiles.total * p.split : min(sms / 2, sh.tiles.total);
+  return (int)launch_pdl_cluster(gemm_int8_pair_kernel<SPLIT>, dim3(2 * pairs), dim3(THREADS), SPLIT ? 2u * p.split : 2u, P_SMEM, st, p,
+                                 sh, tw, tx);
 }
 
 template <int BN>
@@ -729,21 +638,9 @@ int launch(const I8Params& p, int dev, const CUtensorMap& tw, const CUtensorMap&
 }
 }  // namespace
 
-// Bytes of `work` (16-byte aligned) that vg_gemm_int8 needs for this shape on the current device; 0 for most. Negative: error.
-extern "C" long long vg_gemm_int8_work_bytes(int M, int K, int N) {
-  if (M <= 0 || K <= 0 || N <= NARROW_MAX) return 0;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return -1;
-  const Room* room = room_of(dev);
-  if (!room) return -3;
-  PairShape sh{};
-  choose_pair(N, (K + BK - 1) / BK, (M + 2 * BM - 1) / (2 * BM), room->sms, &sh);
-  return pair_work_bytes(sh);
-}
-
 extern "C" int vg_gemm_int8(const void* codes, long long ldw, const float* sw, const void* q, long long ldq, const float* sx,
-                            void* out, long long ldo, int out_f32, int M, int K, int N, void* work, long long work_bytes, int* err, cudaStream_t st) {
-  if (M <= 0 || N < 0 || K <= 0 || K > 131071 || (long long)M * N > (1ll << 40) || M > (1 << 26) || N > (1 << 27) || ldw % 16 || ldq % 16 || ldw < K || ldq < K || ldo < M ||
+                            void* out, long long ldo, int out_f32, int M, int K, int N, int* err, cudaStream_t st) {
+  if (M <= 0 || N < 0 || K <= 0 || K > 131071 || ldw % 16 || ldq % 16 || ldw < K || ldq < K || ldo < M ||
       (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(q)) % 16)
     return -2;
   if (N == 0) return 0;
@@ -760,9 +657,10 @@ extern "C" int vg_gemm_int8(const void* codes, long long ldw, const float* sw, c
   CUtensorMap tw, tx;
   int rc = make_map(codes, M, K, ldw, BM, &tw);
   if (rc) return rc;
-  if (N <= NARROW_MAX) {
+  if (N <= 64) {
     const int bn = N <= 16 ? 16 : N <= 32 ? 32 : 64;
     const int tiles = (M + BM - 1) / BM;
+    if (tiles > (1 << 26)) return -2;
     // The widest split whose clusters all run at once, two CTAs per SM, with four slabs per CTA at least. 16 x 5120 x
     // 17408 (40 tiles): 31.8 us unsplit, 20.6 / 19.5 / 17.3 with 2 / 3 / 6 parts, 23.1 with 7 (a second wave).
     for (int s = 2; s <= MAX_SPLIT && s <= slabs / 4; ++s)
@@ -776,14 +674,13 @@ extern "C" int vg_gemm_int8(const void* codes, long long ldw, const float* sw, c
     }
   }
   PairShape sh{};
-  choose_pair(N, slabs, (M + 2 * BM - 1) / (2 * BM), room->sms, &sh);
-  if (sh.shared && work_bytes >= pair_work_bytes(sh)) {
-    sh.count = static_cast<uint32_t*>(work);
-    sh.work = reinterpret_cast<uint4*>(static_cast<char*>(work) + pair_count_bytes(sh));
-  } else if (sh.shared) {
-    return -4;
-  }
+  sh.tiles.mt = (M + 2 * BM - 1) / (2 * BM);
+  choose_pair(N, slabs, *room, &sh, &p.split);
+  sh.stage = A_BYTES + sh.bn / 2 * BK;
+  sh.stages = min(P_MAX_STAGES, P_RING / sh.stage);
+  if ((long long)sh.tiles.mt * sh.tiles.nt > (1 << 26)) return -2;
+  sh.tiles.total = sh.tiles.mt * sh.tiles.nt;
   rc = make_map(q, N, K, ldq, sh.bn / 2, &tx);
   if (rc) return rc;
-  return launch_pair(p, sh, dev, tw, tx, st);
+  return p.split > 1 ? launch_pair<true>(p, sh, room->sms, dev, tw, tx, st) : launch_pair<false>(p, sh, room->sms, dev, tw, tx, st);
 }

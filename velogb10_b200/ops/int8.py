@@ -12,7 +12,6 @@ tensors' device, and allocate only what the caller does not hand in. Rows ``>= n
 """
 from __future__ import annotations
 
-import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -53,24 +52,23 @@ def _fn(name: str):
                  "vg_swiglu_int8": (P, L, I, I, P, L, P, P),
                  "vg_add_rmsnorm_int8": (P, L, P, L, P, I, I, F, I, P, L, P, P, L, P),
                  "vg_dequant_int8": (P, L, P, P, L, I, I, I, P),
-                 "vg_gemm_int8": (P, L, P, P, L, P, P, L, I, I, I, I, P, L, P, P),
-                 "vg_gemm_int8_work_bytes": (I, I, I)}[name]
+                 "vg_gemm_int8": (P, L, P, P, L, P, P, L, I, I, I, I, P, P)}[name]
         f = getattr(_lib.lib(), name)
         f.argtypes = types
-        f.restype = c_ll if name.endswith("_bytes") else c_int
+        f.restype = c_int
         _fns[name] = f
     return f
 
 
-def _launch(name: str, device: torch.device, *args, kernels: int = 1):
+def _launch(name: str, device: torch.device, *args):
     index = device.index
     if index is None or device.type != "cuda":
         raise KernelError(f"{name[3:]} runs on CUDA tensors, got {device}")
     if index == torch.cuda.current_device():
-        _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name, kernels)
+        _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name)
         return
     with torch.cuda.device(index):
-        _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name, kernels)
+        _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name)
 
 
 def _rows(t: torch.Tensor, n: Optional[int], what: str) -> int:
@@ -181,15 +179,6 @@ def dequantize_act_int8(act: Int8Act, n: Optional[int] = None, out: Optional[tor
     return out
 
 
-@functools.lru_cache(maxsize=4096)
-def _work_bytes(m: int, k: int, n: int, index: int) -> int:
-    with torch.cuda.device(index):
-        b = _fn("vg_gemm_int8_work_bytes")(m, k, n)
-    if b < 0:
-        raise KernelError(f"vg_gemm_int8_work_bytes failed with code {b}")
-    return b
-
-
 def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional[torch.Tensor] = None,
                 out_f32: bool = False) -> torch.Tensor:
     """``out[:n] = act @ W^T`` for an ``int8`` linear, bf16 or fp32 (``out``'s type when it is given). Codes of both sides are
@@ -217,13 +206,6 @@ def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional
     else:
         ldo = _matrix(out, "out", (torch.bfloat16, torch.float32), n, m, dev)
     if n:
-        if dev.type != "cuda":
-            raise KernelError(f"gemm_int8 runs on CUDA tensors, got {dev}")
-        # partial sums of tiles whose K is cut over several CTA pairs: scratch of this call, so that calls on other streams
-        # and captured graphs never share it
-        size = _work_bytes(m, k, n, dev.index) if n > 64 else 0
-        work = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
         _launch("vg_gemm_int8", dev, wp, ldw, q.row_scale.data_ptr(), qp, ldq, act.scale.data_ptr(), out.data_ptr(), ldo,
-                1 if out.dtype == torch.float32 else 0, m, k, n, work.data_ptr() if size else 0, size, _lib.err_word(dev).data_ptr(),
-                kernels=2 if size else 1)
+                1 if out.dtype == torch.float32 else 0, m, k, n, _lib.err_word(dev).data_ptr() if dev.type == "cuda" else 0)
     return out
