@@ -97,11 +97,12 @@ int vg_gemm_simt(const void* wq, const void* scales, const float* row_scale, con
 // (scale NaN and codes 0 for a row that holds an infinity or a NaN); k <= 131072. dtype: 0 bf16, 1 f16, 2 f32.
 // vg_gemm_int8: out[n, m] = (sum_k q[n, k] codes[m, k]) * sx[n] * sw[m]; K <= 131071, code rows on 16-byte boundaries.
 int vg_quant_int8(const void* x, long long ldx, int dtype, int n, int k, void* q, long long ldq, float* scale,
-                  cudaStream_t stream);
-int vg_swiglu_int8(const void* gu, long long ldx, int n, int inter, void* q, long long ldq, float* scale, cudaStream_t stream);
+                  int* err, cudaStream_t stream);
+int vg_swiglu_int8(const void* gu, long long ldx, int n, int inter, void* q, long long ldq, float* scale, int* err,
+                   cudaStream_t stream);
 int vg_add_rmsnorm_int8(void* res, long long ld_res, const void* delta, long long ld_delta, const float* w, int n, int h,
                         float eps, int plus_one, void* q, long long ldq, float* scale, void* out16, long long ld_out16,
-                        cudaStream_t stream);
+                        int* err, cudaStream_t stream);
 int vg_dequant_int8(const void* q, long long ldq, const float* scale, void* out, long long ldo, int dtype, int n, int k,
                     cudaStream_t stream);
 int vg_gemm_int8(const void* codes, long long ldw, const float* sw, const void* q, long long ldq, const float* sx, void* out,

@@ -11,6 +11,8 @@
 // inputs and outputs once and nothing else. A row that holds an infinity or a NaN (or whose sum of squares leaves
 // fp32) gets scale NaN and codes 0: everything computed from it is NaN instead of a plausible wrong number. The floor
 // of the scale keeps an all-zero row at codes 0 and 1 / s finite.
+#include <atomic>
+
 #include "common.cuh"
 #include "api.h"
 
@@ -18,6 +20,7 @@ namespace {
 using namespace vg;
 
 constexpr int MAX_CLUSTER = 8;
+constexpr int RING_SLOTS = 8;
 constexpr float INT8_MAX_CODE = 127.0f;
 constexpr float SCALE_FLOOR = 7.52316384526264e-37f;      // 2^-120
 
@@ -33,6 +36,7 @@ struct RowParams {
   __half* out16;                 // norm only, may be null
   int k, cluster;
   float eps, w_off;
+  int* err;
 };
 
 VG_DEVINL void dsmem_st_f32x2(uint32_t addr, float a, float b) {
@@ -52,6 +56,63 @@ VG_DEVINL void block_reduce(unsigned& mx, float& sum, unsigned* red_m, float* re
   __syncthreads();
   mx = __reduce_max_sync(0xffffffffu, lane < nw ? red_m[lane] : 0u);
   if (SUM) sum = warp_sum(lane < nw ? red_s[lane] : 0.f);
+}
+
+// Eight values -> eight codes, rint(v * f) for |v * f| < 2^22: adding 1.5 * 2^23 leaves the rounded integer in the low bits
+// of the sum. (cvt.rni runs at an eighth of the rate, next to the exponentials.)
+VG_DEVINL uint2 codes8(const float* v, float f) {
+  uint32_t t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = __float_as_uint(__fmaf_rn(v[i], f, 12582912.0f));
+  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
+}
+VG_DEVINL void unpack8(uint4 a, float* v, bool f16) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = (&a.x)[i];
+    const float2 f = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w))
+                         : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+VG_DEVINL uint4 pack_bf16(const float* v) {
+  uint4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    (&o.x)[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return o;
+}
+VG_DEVINL uint4 pack_f16_sat(const float* v) {
+  uint4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __halves2half2(f32_to_f16_sat(v[2 * i]), f32_to_f16_sat(v[2 * i + 1]));
+    (&o.x)[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return o;
+}
+
+// What a row's statistics give: the scale, its reciprocal and (norm) 1 / rms.
+struct RowScale {
+  float s, f, inv;
+  bool bad;
+};
+template <int KIND>
+VG_DEVINL RowScale row_scale(const RowParams& p, unsigned mx, float ss) {
+  // The norm's factor 1 / rms is common to the row, so the maximum of |res * w| found in the same pass as the sum of
+  // squares is enough: one reduction instead of two.
+  RowScale o;
+  o.inv = KIND == ROW_NORM ? rsqrtf(ss / (float)p.k + p.eps) : 1.f;
+  const float amax = __uint_as_float(mx) * o.inv;
+  o.bad = !(amax < INFINITY) || (KIND == ROW_NORM && !(ss < INFINITY));
+  o.s = o.bad ? __uint_as_float(0x7fffffffu) : fmaxf(__fdiv_rn(amax, INT8_MAX_CODE), SCALE_FLOOR);
+  // codes are rint(y * (1 / s)): |y| / s <= 127 (1 + 2^-22), which rounds to 127 at most; 1 / s <= 2^120
+  o.f = o.bad ? 0.f : __fdiv_rn(1.f, o.s);
+  return o;
 }
 
 template <int KIND>
@@ -183,40 +244,26 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
     }
   }
 
-  // The norm's factor 1 / rms is common to the row, so the maximum of |res * w| found in the same pass as the sum of
-  // squares is enough: one reduction instead of two.
-  const float amax = __uint_as_float(mx);
-  float inv = 1.f;
-  bool bad = mx >= 0x7f800000u;
+  const RowScale rs = row_scale<KIND>(p, mx, ss);
+  if (tid == 0) p.scale[row] = rs.s;
   if (KIND == ROW_NORM) {
-    bad |= !(ss < INFINITY);
-    inv = rsqrtf(ss / (float)k + p.eps);
+#pragma unroll
+    for (int c = 0; c < MAXC; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[c][i] *= rs.inv;
   }
-  const float s = bad ? __uint_as_float(0x7fffffffu) : fmaxf(__fdiv_rn(amax * inv, INT8_MAX_CODE), SCALE_FLOOR);
-  // rint(y * (inv / s)): |y| * inv / s <= 127 (1 + 2^-22), which rounds to 127 at most
-  const float f = bad ? 0.f : __fdiv_rn(inv, s);
-  if (tid == 0) p.scale[row] = s;
   signed char* q = p.q + row * p.ldq;
 #pragma unroll
   for (int c = 0; c < MAXC; ++c) {
     if (VEC) {
       const int e = (tid + c * T) * 8;
       if (e < k) {
-        uint2 o;
-        unsigned* ow = reinterpret_cast<unsigned*>(&o);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          int b[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) b[i] = bad ? 0 : __float2int_rn(v[c][4 * j + i] * f);
-          ow[j] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-        }
-        *reinterpret_cast<uint2*>(q + e) = o;
+        *reinterpret_cast<uint2*>(q + e) = rs.bad ? make_uint2(0u, 0u) : codes8(v[c], rs.f);
         if (KIND == ROW_NORM && p.out16) {
           uint4 h4;
           __half* h = reinterpret_cast<__half*>(&h4);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = bad ? __ushort_as_half(0x7fff) : f32_to_f16_sat(v[c][i] * inv);
+          for (int i = 0; i < 8; ++i) h[i] = rs.bad ? __ushort_as_half(0x7fff) : f32_to_f16_sat(v[c][i]);
           *reinterpret_cast<uint4*>(p.out16 + row * p.ldo + e) = h4;
         }
       }
@@ -225,13 +272,121 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
       for (int i = 0; i < 8; ++i) {
         const int e = tid + (c * 8 + i) * T;
         if (e < k) {
-          q[e] = (signed char)(bad ? 0 : __float2int_rn(v[c][i] * f));
+          q[e] = (signed char)(rs.bad ? 0 : __float2int_rn(v[c][i] * rs.f));
           if (KIND == ROW_NORM && p.out16)
-            p.out16[row * p.ldo + e] = bad ? __ushort_as_half(0x7fff) : f32_to_f16_sat(v[c][i] * inv);
+            p.out16[row * p.ldo + e] = rs.bad ? __ushort_as_half(0x7fff) : f32_to_f16_sat(v[c][i]);
         }
       }
     }
   }
+}
+
+// Many rows: persistent blocks with a ring of whole rows in shared memory, filled by bulk copies several rows ahead, so
+// the memory system stays busy while a block reduces, quantises and stores. A row's slot is refilled as soon as the
+// reduction's barrier has shown that every thread holds its part in registers: one barrier per row.
+template <int KIND, int MAXC>
+__global__ void __launch_bounds__(MAXC == 4 ? 640 : 1024) row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ __align__(8) uint64_t full[RING_SLOTS];
+  __shared__ unsigned red_m[2][32];
+  __shared__ float red_s[2][32];
+  __shared__ int stuck;
+  constexpr int ES = KIND == ROW_F32 ? 4 : 2;
+  pdl_trigger();
+  const int k = p.k, T = blockDim.x, step = gridDim.x;
+  const uint32_t x_bytes = (uint32_t)k * ES * (KIND == ROW_SWIGLU ? 2 : 1);
+  const bool two = KIND == ROW_NORM && p.delta;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < slots; ++i) mbar_init(full + i, 1);
+    stuck = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  auto fill = [&](int slot, size_t row) {
+    uint8_t* dst = ring + (size_t)slot * slot_bytes;
+    mbar_arrive_expect_tx(full + slot, two ? 2 * x_bytes : x_bytes);
+    tma_bulk_g2s(dst, static_cast<const char*>(p.x) + row * p.ldx * ES, x_bytes, full + slot);
+    if (two) tma_bulk_g2s(dst + x_bytes, p.delta + row * p.ldd, x_bytes, full + slot);
+  };
+  pdl_wait();
+  if (threadIdx.x == 0)
+    for (int i = 0; i < slots && (int)blockIdx.x + i * step < n; ++i) fill(i, blockIdx.x + (size_t)i * step);
+  int slot = 0, it = 0;
+  uint32_t ph = 0;
+  for (int row = blockIdx.x; row < n; row += step, ++it) {
+    if (!mbar_wait(full + slot, ph)) {
+      if (p.err) atomicCAS(p.err, 0, (int)VG_ERR_TMA_WAIT);
+      stuck = 1;
+    }
+    const uint8_t* src = ring + (size_t)slot * slot_bytes;
+    float v[MAXC][8];
+    unsigned mx = 0;
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < MAXC; ++c) {
+      const int e = (threadIdx.x + c * T) * 8;
+      if (e < k) {
+        if (KIND == ROW_F32) {
+          *reinterpret_cast<float4*>(v[c]) = *reinterpret_cast<const float4*>(src + (size_t)e * 4);
+          *reinterpret_cast<float4*>(v[c] + 4) = *reinterpret_cast<const float4*>(src + (size_t)e * 4 + 16);
+        } else {
+          unpack8(*reinterpret_cast<const uint4*>(src + (size_t)e * 2), v[c], KIND == ROW_F16);
+        }
+        if (KIND == ROW_SWIGLU) {
+          float u[8];
+          unpack8(*reinterpret_cast<const uint4*>(src + (size_t)(k + e) * 2), u, false);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[c][i] = silu(v[c][i]) * u[i];
+        }
+        if (two) {
+          float d[8];
+          unpack8(*reinterpret_cast<const uint4*>(src + x_bytes + (size_t)e * 2), d, false);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] += v[c][i];
+          const uint4 r4 = pack_bf16(d);
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(const_cast<void*>(p.x)) + row * p.ldx + e) = r4;
+          unpack8(r4, v[c], false);
+        }
+        if (KIND == ROW_NORM) {
+          const float4 w0 = __ldg(reinterpret_cast<const float4*>(p.w + e)), w1 = __ldg(reinterpret_cast<const float4*>(p.w + e + 4));
+          const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            ss += v[c][i] * v[c][i];
+            v[c][i] *= ww[i] + p.w_off;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(v[c][i]) & 0x7fffffffu);
+    }
+    block_reduce<KIND == ROW_NORM>(mx, ss, red_m[it & 1], red_s[it & 1]);
+    if (stuck) break;                                      // seen by every thread: set before the barrier
+    if (threadIdx.x == 0 && row + (long long)slots * step < n) fill(slot, row + (size_t)slots * step);
+    const RowScale rs = row_scale<KIND>(p, mx, ss);
+    if (threadIdx.x == 0) p.scale[row] = rs.s;
+#pragma unroll
+    for (int c = 0; c < MAXC; ++c) {
+      const int e = (threadIdx.x + c * T) * 8;
+      if (e < k) {
+        if (KIND == ROW_NORM) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[c][i] *= rs.inv;
+        }
+        *reinterpret_cast<uint2*>(p.q + (size_t)row * p.ldq + e) = rs.bad ? make_uint2(0u, 0u) : codes8(v[c], rs.f);
+        if (KIND == ROW_NORM && p.out16) {
+          const uint4 nan4 = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+          *reinterpret_cast<uint4*>(p.out16 + (size_t)row * p.ldo + e) = rs.bad ? nan4 : pack_f16_sat(v[c]);
+        }
+      }
+    }
+    if (++slot == slots) { slot = 0; ph ^= 1; }
+  }
+  if (stuck && threadIdx.x == 0)
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);        // let copies in flight land before the block ends
 }
 
 template <typename OUT>
@@ -267,6 +422,10 @@ __global__ void __launch_bounds__(256) dequant_int8_kernel(const signed char* __
   }
 }
 
+constexpr int RING_BYTES = 200 * 1024;            // ring of all blocks of an SM
+constexpr int RING_PER_SM = 4;                    // blocks per SM
+constexpr int RING_MIN_ROWS = 2;                  // rows per SM from which the ring form pays
+
 // Largest row width: a cluster of eight CTAs of 1024 threads with two groups of eight each.
 constexpr int ROW_MAX = MAX_CLUSTER * 1024 * 2 * 8;
 
@@ -283,6 +442,33 @@ cudaError_t launch_shape(RowParams p, int n, cudaStream_t st) {
   return launch_pdl_cluster(row_int8_kernel<KIND, VEC, 2, true>, dim3(n * p.cluster), dim3((t + 31) / 32 * 32), p.cluster, 0, st, p);
 }
 
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  n = known[dev & 63].load();
+  if (n <= 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev & 63].store(n);
+  return n;
+}
+
+template <int KIND, int MAXC>
+int launch_ring(const RowParams& p, int n, int slot_bytes, int sms, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (!(done.load() & (1ull << (dev & 63)))) {
+    e = cudaFuncSetAttribute(row_int8_ring_kernel<KIND, MAXC>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES);
+    if (e != cudaSuccess) return (int)e;
+    done.fetch_or(1ull << (dev & 63));
+  }
+  const int groups = p.k / 8, threads = ((groups + MAXC - 1) / MAXC + 31) / 32 * 32;
+  const int per_sm = max(1, min(min(RING_PER_SM, 1536 / threads), RING_BYTES / (2 * slot_bytes)));
+  const int slots = max(2, min(RING_SLOTS, RING_BYTES / per_sm / slot_bytes));
+  const int grid = min(n, sms * per_sm);
+  return (int)launch_pdl(row_int8_ring_kernel<KIND, MAXC>, dim3(grid), dim3(threads), (size_t)slots * slot_bytes, st, p, n, slots, slot_bytes);
+}
+
 // `esize`: bytes of one input element; the wide path wants whole groups of eight and 16-byte addresses on every row
 template <int KIND>
 int launch_row(const RowParams& p, int n, int esize, cudaStream_t st) {
@@ -294,6 +480,13 @@ int launch_row(const RowParams& p, int n, int esize, cudaStream_t st) {
     vec = vec && aligned(p.w, 16);
     if (p.delta) vec = vec && aligned(p.delta, 16) && (n == 1 || p.ldd % 8 == 0);
     if (p.out16) vec = vec && aligned(p.out16, 16) && (n == 1 || p.ldo % 8 == 0);
+  }
+  const int sms = sm_count(), slot = p.k * esize * ((KIND == ROW_SWIGLU || p.delta) ? 2 : 1);
+  if (vec && n >= RING_MIN_ROWS * sms && slot % 16 == 0 && 2 * slot <= RING_BYTES && p.k <= 640 * 32) {
+    const int groups = p.k / 8;
+    return groups <= 32 ? launch_ring<KIND, 1>(p, n, slot, sms, st)
+           : groups <= 1024 ? launch_ring<KIND, 2>(p, n, slot, sms, st)
+                            : launch_ring<KIND, 4>(p, n, slot, sms, st);
   }
   const cudaError_t e = vec ? launch_shape<KIND, true>(p, n, st) : launch_shape<KIND, false>(p, n, st);
   return (int)e;
@@ -312,9 +505,9 @@ int launch_dequant(const signed char* q, long long ldq, const float* scale, void
 }  // namespace
 
 extern "C" int vg_quant_int8(const void* x, long long ldx, int dtype, int n, int k, void* q, long long ldq, float* scale,
-                             cudaStream_t st) {
+                             int* err, cudaStream_t st) {
   RowParams p{};
-  p.x = x; p.ldx = ldx; p.k = k; p.q = static_cast<signed char*>(q); p.ldq = ldq; p.scale = scale;
+  p.x = x; p.ldx = ldx; p.k = k; p.q = static_cast<signed char*>(q); p.ldq = ldq; p.scale = scale; p.err = err;
   switch (dtype) {
     case ROW_BF16: return launch_row<ROW_BF16>(p, n, 2, st);
     case ROW_F16: return launch_row<ROW_F16>(p, n, 2, st);
@@ -324,18 +517,18 @@ extern "C" int vg_quant_int8(const void* x, long long ldx, int dtype, int n, int
 }
 
 extern "C" int vg_swiglu_int8(const void* gu, long long ldx, int n, int inter, void* q, long long ldq, float* scale,
-                              cudaStream_t st) {
+                              int* err, cudaStream_t st) {
   RowParams p{};
-  p.x = gu; p.ldx = ldx; p.k = inter; p.q = static_cast<signed char*>(q); p.ldq = ldq; p.scale = scale;
+  p.x = gu; p.ldx = ldx; p.k = inter; p.q = static_cast<signed char*>(q); p.ldq = ldq; p.scale = scale; p.err = err;
   return launch_row<ROW_SWIGLU>(p, n, 2, st);
 }
 
 extern "C" int vg_add_rmsnorm_int8(void* res, long long ld_res, const void* delta, long long ld_delta, const float* w, int n,
                                    int h, float eps, int plus_one, void* q, long long ldq, float* scale, void* out16,
-                                   long long ld_out16, cudaStream_t st) {
+                                   long long ld_out16, int* err, cudaStream_t st) {
   RowParams p{};
   p.x = res; p.ldx = ld_res; p.delta = static_cast<const __nv_bfloat16*>(delta); p.ldd = ld_delta; p.w = w; p.k = h;
-  p.eps = eps; p.w_off = plus_one ? 1.0f : 0.0f; p.q = static_cast<signed char*>(q); p.ldq = ldq; p.scale = scale;
+  p.eps = eps; p.w_off = plus_one ? 1.0f : 0.0f; p.q = static_cast<signed char*>(q); p.ldq = ldq; p.scale = scale; p.err = err;
   p.out16 = static_cast<__half*>(out16); p.ldo = ld_out16;
   return launch_row<ROW_NORM>(p, n, 2, st);
 }

@@ -48,9 +48,9 @@ def _fn(name: str):
     f = _fns.get(name)
     if f is None:
         P, I, L, F = c_void_p, c_int, c_ll, c_float
-        types = {"vg_quant_int8": (P, L, I, I, I, P, L, P, P),
-                 "vg_swiglu_int8": (P, L, I, I, P, L, P, P),
-                 "vg_add_rmsnorm_int8": (P, L, P, L, P, I, I, F, I, P, L, P, P, L, P),
+        types = {"vg_quant_int8": (P, L, I, I, I, P, L, P, P, P),
+                 "vg_swiglu_int8": (P, L, I, I, P, L, P, P, P),
+                 "vg_add_rmsnorm_int8": (P, L, P, L, P, I, I, F, I, P, L, P, P, L, P, P),
                  "vg_dequant_int8": (P, L, P, P, L, I, I, I, P),
                  "vg_gemm_int8": (P, L, P, P, L, P, P, L, I, I, I, I, P, P)}[name]
         f = getattr(_lib.lib(), name)
@@ -69,6 +69,10 @@ def _launch(name: str, device: torch.device, *args):
         return
     with torch.cuda.device(index):
         _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name)
+
+
+def _err(device: torch.device) -> int:
+    return _lib.err_word(device).data_ptr() if device.type == "cuda" else 0
 
 
 def _rows(t: torch.Tensor, n: Optional[int], what: str) -> int:
@@ -121,7 +125,7 @@ def quantize_act_int8(x: torch.Tensor, n: Optional[int] = None, out: Optional[In
     out, ldq = _out(out, n, k, dev)
     ld = _matrix(x, "x", _DTYPE, n, k)
     if n:
-        _launch("vg_quant_int8", dev, x.data_ptr(), ld, _DTYPE[x.dtype], n, k, out.q.data_ptr(), ldq, out.scale.data_ptr())
+        _launch("vg_quant_int8", dev, x.data_ptr(), ld, _DTYPE[x.dtype], n, k, out.q.data_ptr(), ldq, out.scale.data_ptr(), _err(dev))
     return out
 
 
@@ -133,7 +137,7 @@ def swiglu_int8(gu: torch.Tensor, n: Optional[int] = None, inter: Optional[int] 
     ld = _matrix(gu, "gu", (torch.bfloat16,), n, 2 * inter)
     out, ldq = _out(out, n, inter, gu.device)
     if n:
-        _launch("vg_swiglu_int8", gu.device, gu.data_ptr(), ld, n, inter, out.q.data_ptr(), ldq, out.scale.data_ptr())
+        _launch("vg_swiglu_int8", gu.device, gu.data_ptr(), ld, n, inter, out.q.data_ptr(), ldq, out.scale.data_ptr(), _err(gu.device))
     return out
 
 
@@ -156,7 +160,7 @@ def add_rmsnorm_int8(res: torch.Tensor, delta: Optional[torch.Tensor], w: torch.
     if n:
         _launch("vg_add_rmsnorm_int8", dev, res.data_ptr(), ld, 0 if delta is None else delta.data_ptr(), ldd, w.data_ptr(), n, h,
                 eps, 1 if plus_one else 0, out.q.data_ptr(), ldq, out.scale.data_ptr(),
-                0 if out16 is None else out16.data_ptr(), ldo)
+                0 if out16 is None else out16.data_ptr(), ldo, _err(dev))
     return out
 
 
@@ -207,5 +211,5 @@ def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional
         ldo = _matrix(out, "out", (torch.bfloat16, torch.float32), n, m, dev)
     if n:
         _launch("vg_gemm_int8", dev, wp, ldw, q.row_scale.data_ptr(), qp, ldq, act.scale.data_ptr(), out.data_ptr(), ldo,
-                1 if out.dtype == torch.float32 else 0, m, k, n, _lib.err_word(dev).data_ptr() if dev.type == "cuda" else 0)
+                1 if out.dtype == torch.float32 else 0, m, k, n, _err(dev))
     return out
