@@ -39,21 +39,28 @@ struct RowParams {
   int* err;
 };
 
+// max(|m|, |a|, |b|), NaN if one of them is
+VG_DEVINL float max_abs3(float m, float a, float b) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
+  return r;
+}
 VG_DEVINL void dsmem_st_f32x2(uint32_t addr, float a, float b) {
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
 }
 
-// Block-wide maximum of a non-negative float's bits (so NaN > inf > finite) and sum, one barrier.
+// Maximum of a non-negative float's bits (so NaN > inf > finite) and sum over `threads` threads of which this is number
+// `tid`, one barrier: the block's, or named barrier `bar` of a team.
 template <bool SUM>
-VG_DEVINL void block_reduce(unsigned& mx, float& sum, unsigned* red_m, float* red_s) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+VG_DEVINL void block_reduce(unsigned& mx, float& sum, unsigned* red_m, float* red_s, int tid, int threads, int bar = 0) {
+  const int lane = tid & 31, w = tid >> 5, nw = threads >> 5;
   mx = __reduce_max_sync(0xffffffffu, mx);
   if (SUM) sum = warp_sum(sum);
   if (lane == 0) {
     red_m[w] = mx;
     if (SUM) red_s[w] = sum;
   }
-  __syncthreads();
+  asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory");
   mx = __reduce_max_sync(0xffffffffu, lane < nw ? red_m[lane] : 0u);
   if (SUM) sum = warp_sum(lane < nw ? red_s[lane] : 0.f);
 }
@@ -115,46 +122,94 @@ VG_DEVINL RowScale row_scale(const RowParams& p, unsigned mx, float ss) {
   return o;
 }
 
-template <int KIND>
-VG_DEVINL float load_one(const RowParams& p, size_t row, int e) {
-  if (KIND == ROW_F32) return static_cast<const float*>(p.x)[row * p.ldx + e];
-  if (KIND == ROW_F16) return __half2float(static_cast<const __half*>(p.x)[row * p.ldx + e]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p.x)[row * p.ldx + e]);
-}
-
-template <int KIND>
-VG_DEVINL void load_eight(const RowParams& p, size_t row, int e, float* v) {
-  if (KIND == ROW_F32) {
-    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + row * p.ldx + e);
-    const float4 a = s[0], b = s[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else if (KIND == ROW_F16) {
-    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.x) + row * p.ldx + e);
-    const __half2* h = reinterpret_cast<const __half2*>(&a);
+// Eight elements from element e of a row that starts at `base` and has `limit` of them in memory, as packed words; those
+// before `lo` and from `left` on are zero. VEC: 16-byte addresses and whole groups. Else the address may be anything a
+// tensor of that type can have: the aligned words around the group are loaded and shifted into place (by the same amount
+// in a whole row), as long as they lie inside the row; the edges are read one by one.
+template <bool VEC, int ES>
+VG_DEVINL void load8_raw(const char* base, long long e, int lo, int left, long long limit, uint32_t* w) {
+  constexpr int W = 2 * ES;
+  const char* a = base + e * ES;
+  if (VEC) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(h[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+    for (int i = 0; i < W / 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = *reinterpret_cast<const uint4*>(a + 16 * i);
+    return;
+  }
+  const uint32_t mis = (uint32_t)(reinterpret_cast<uintptr_t>(a) & 15);
+  const char* a0 = a - mis;
+  if (lo == 0 && left >= 8 && (mis == 0 || (a0 >= base && a0 + W * 4 + 16 <= base + limit * ES))) {
+    uint32_t t[W + 4] = {};
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) *reinterpret_cast<uint4*>(t + 4 * i) = *reinterpret_cast<const uint4*>(a0 + 16 * i);
+    if (mis) *reinterpret_cast<uint4*>(t + W) = *reinterpret_cast<const uint4*>(a0 + W * 4);
+    if (mis & 8) {
+#pragma unroll
+      for (int i = 0; i < W + 2; ++i) t[i] = t[i + 2];
     }
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x) + row * p.ldx + e);
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&a);
+    if (mis & 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __bfloat1622float2(h[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+      for (int i = 0; i < W + 1; ++i) t[i] = t[i + 1];
+    }
+    if (ES == 2 && (mis & 2)) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) t[i] = __funnelshift_r(t[i], t[i + 1], 16);
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = t[i];
+    return;
+  }
+  if (ES == 4) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = i >= lo && i < left ? *reinterpret_cast<const uint32_t*>(a + 4 * i) : 0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const uint32_t l = i >= lo && i < left ? *reinterpret_cast<const uint16_t*>(a + 2 * i) : 0u;
+      const uint32_t h = i + 1 >= lo && i + 1 < left ? *reinterpret_cast<const uint16_t*>(a + 2 * i + 2) : 0u;
+      w[i / 2] = l | (h << 16);
     }
   }
 }
+// Eight 2-byte values of a group to memory: at once where the address and the row's ends allow it.
+template <bool VEC>
+VG_DEVINL void store8_half(void* dst, int lo, int left, uint4 v) {
+  if (VEC || (lo == 0 && left >= 8 && reinterpret_cast<uintptr_t>(dst) % 16 == 0)) {
+    *reinterpret_cast<uint4*>(dst) = v;
+    return;
+  }
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i >= lo && i < left) static_cast<uint16_t*>(dst)[i] = (uint16_t)((&v.x)[i >> 1] >> (16 * (i & 1)));
+  }
+}
+// The codes of group [e, e + 8) of a row of k, where groups start `shift` elements past multiples of eight: the 8-byte
+// word at the next multiple takes the rest from the next lane (lane 31 only hands its codes over). What is left at the
+// row's ends, and everything when the row of codes is not 8-byte aligned, is written byte by byte. All lanes call this.
+VG_DEVINL void store_codes_shifted(signed char* q, int e, int k, int shift, uint2 v) {
+  const unsigned long long own = ((unsigned long long)v.y << 32) | v.x;
+  const unsigned long long next = __shfl_down_sync(0xffffffffu, own, 1);
+  if ((threadIdx.x & 31) == 31 || e >= k) return;
+  const bool wide = reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  const int word = shift ? e + 8 - shift : e;                        // first multiple of eight inside or after the group's start
+  const bool full = wide && word >= 0 && word + 8 <= k;
+  const bool lead_done = shift == 0 || (wide && word >= 8 && word <= k);          // by the previous lane's word
+  if (full) *reinterpret_cast<unsigned long long*>(q + word) = shift ? (own >> (8 * (8 - shift))) | (next << (8 * shift)) : own;
+  if (full && lead_done) return;
+  for (int i = 0; i < 8; ++i)
+    if (!(i < word - e ? lead_done : full) && e + i >= 0 && e + i < k) q[e + i] = (signed char)(own >> (8 * i));
+}
 
 // A row belongs to one CTA, or (CL) to a cluster of them that exchanges its partial statistics through distributed
-// shared memory. A thread owns MAXC groups of eight elements: consecutive ones with 16-byte accesses (VEC), or strided
-// by all the row's threads with single accesses where the width or an address does not allow that.
+// shared memory. A thread owns MAXC groups of eight consecutive elements; all its loads are issued before the first use.
+// Rows that do not all start on 16-byte boundaries (!VEC) are cut into groups at the boundaries of x, so x is read and
+// written back in whole words whatever the width; the codes are shifted into their own words on the way out, with a lane's
+// neighbour supplying the rest. Warps overlap by one group for that: lane 31 repeats the next warp's first. (Bytes stored
+// one by one at the seams of warps: 11.7 us at 1237 x 4111, with the overlap 8.7.)
 template <int KIND, bool VEC, int MAXC, bool CL>
 __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
+  constexpr int ES = KIND == ROW_F32 ? 4 : 2;
+  constexpr bool PAIR = KIND == ROW_SWIGLU || KIND == ROW_NORM;
   __shared__ unsigned red_m[32];
   __shared__ float red_s[32];
   __shared__ float2 peer[MAX_CLUSTER];
@@ -167,71 +222,65 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
   const int T = blockDim.x * nrank;
   const int tid = threadIdx.x + rank * blockDim.x;
   const int k = p.k;
-  float v[MAXC][8];
-  unsigned mx = 0;
-  float ss = 0.f;
+  char* x_row = static_cast<char*>(const_cast<void*>(p.x)) + row * p.ldx * ES;
+  const char* d_row = reinterpret_cast<const char*>(p.delta + row * p.ldd);
+  constexpr int LANES = VEC ? 32 : 31;                             // groups of its own that a warp has
+  const int shift = VEC ? 0 : (int)((16 - (reinterpret_cast<uintptr_t>(x_row) & 15)) & 15) / ES;
+  const int e0 = ((tid >> 5) * LANES + (tid & 31)) * 8 - ((8 - shift) & 7), e_step = T / 32 * LANES * 8;
+  const bool owner = VEC || (tid & 31) < 31;
+  uint32_t xr[MAXC][2 * ES], yr[MAXC][4];
 #pragma unroll
   for (int c = 0; c < MAXC; ++c) {
-    if (VEC) {
-      const int e = (tid + c * T) * 8;
-      if (e < k) {
-        load_eight<KIND>(p, row, e, v[c]);
-        if (KIND == ROW_SWIGLU) {
-          float u[8];
-          load_eight<KIND>(p, row, k + e, u);
+    const int e = e0 + c * e_step, lo = max(0, -e);
+    if (e < k) {
+      load8_raw<VEC, ES>(x_row, e, lo, k - e, KIND == ROW_SWIGLU ? 2 * k : k, xr[c]);
+      if (KIND == ROW_SWIGLU) load8_raw<VEC, 2>(x_row, k + e, lo, k - e, 2 * k, yr[c]);
+      if (KIND == ROW_NORM && p.delta) load8_raw<VEC, 2>(d_row, e, lo, k - e, k, yr[c]);
+    }
+  }
+  float v[MAXC][8];
+  float amax = 0.f, ss = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[c][i] = silu(v[c][i]) * u[i];
-        }
-        if (KIND == ROW_NORM && p.delta) {
-          const uint4 d4 = *reinterpret_cast<const uint4*>(p.delta + row * p.ldd + e);
-          const __nv_bfloat16* d = reinterpret_cast<const __nv_bfloat16*>(&d4);
-          uint4 r4;
-          __nv_bfloat16* r = reinterpret_cast<__nv_bfloat16*>(&r4);
+  for (int c = 0; c < MAXC; ++c) {
+    const int e = e0 + c * e_step, lo = max(0, -e);
+    if (e < k) {
+      if (ES == 4) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            r[i] = __float2bfloat16_rn(v[c][i] + __bfloat162float(d[i]));
-            v[c][i] = __bfloat162float(r[i]);
-          }
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(const_cast<void*>(p.x)) + row * p.ldx + e) = r4;
-        }
-        if (KIND == ROW_NORM) {
-          const float4 w0 = *reinterpret_cast<const float4*>(p.w + e), w1 = *reinterpret_cast<const float4*>(p.w + e + 4);
-          const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            ss += v[c][i] * v[c][i];
-            v[c][i] *= ww[i] + p.w_off;
-          }
-        }
+        for (int i = 0; i < 8; ++i) v[c][i] = __uint_as_float(xr[c][i]);
       } else {
+        unpack8(make_uint4(xr[c][0], xr[c][1], xr[c][2], xr[c][3]), v[c], KIND == ROW_F16);
+      }
+      float y[8];
+      if (PAIR) unpack8(make_uint4(yr[c][0], yr[c][1], yr[c][2], yr[c][3]), y, false);
+      if (KIND == ROW_SWIGLU) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
+        for (int i = 0; i < 8; ++i) v[c][i] = silu(v[c][i]) * y[i];
+      }
+      if (KIND == ROW_NORM) {
+        if (p.delta) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] += v[c][i];
+          const uint4 r4 = pack_bf16(y);
+          xr[c][0] = r4.x; xr[c][1] = r4.y; xr[c][2] = r4.z; xr[c][3] = r4.w;      // stored after the reduction
+          unpack8(r4, v[c], false);
+        }
+        uint32_t ww[8];
+        load8_raw<VEC, 4>(reinterpret_cast<const char*>(p.w), e, lo, k - e, k, ww);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ss += owner ? v[c][i] * v[c][i] : 0.f;
+          v[c][i] *= __uint_as_float(ww[i]) + p.w_off;
+        }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = tid + (c * 8 + i) * T;
-        float y = 0.f;
-        if (e < k) {
-          y = load_one<KIND>(p, row, e);
-          if (KIND == ROW_SWIGLU) y = silu(y) * load_one<KIND>(p, row, k + e);
-          if (KIND == ROW_NORM) {
-            if (p.delta) {
-              const __nv_bfloat16 r = __float2bfloat16_rn(y + __bfloat162float(p.delta[row * p.ldd + e]));
-              static_cast<__nv_bfloat16*>(const_cast<void*>(p.x))[row * p.ldx + e] = r;
-              y = __bfloat162float(r);
-            }
-            ss += y * y;
-            y *= p.w[e] + p.w_off;
-          }
-        }
-        v[c][i] = y;
-      }
+      for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(v[c][i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; i += 2) amax = max_abs3(amax, v[c][i], v[c][i + 1]);
   }
-  block_reduce<KIND == ROW_NORM>(mx, ss, red_m, red_s);
+  unsigned mx = __float_as_uint(amax);
+  block_reduce<KIND == ROW_NORM>(mx, ss, red_m, red_s, threadIdx.x, blockDim.x);
   if (CL) {
     cluster_wait();                                   // every CTA of the row has started
     if ((int)threadIdx.x < nrank) dsmem_st_f32x2(dsmem_map(smem_u32(&peer[rank]), threadIdx.x), __uint_as_float(mx), ss);
@@ -252,31 +301,17 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[c][i] *= rs.inv;
   }
-  signed char* q = p.q + row * p.ldq;
+  const uint4 nan4 = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
 #pragma unroll
   for (int c = 0; c < MAXC; ++c) {
-    if (VEC) {
-      const int e = (tid + c * T) * 8;
-      if (e < k) {
-        *reinterpret_cast<uint2*>(q + e) = rs.bad ? make_uint2(0u, 0u) : codes8(v[c], rs.f);
-        if (KIND == ROW_NORM && p.out16) {
-          uint4 h4;
-          __half* h = reinterpret_cast<__half*>(&h4);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = rs.bad ? __ushort_as_half(0x7fff) : f32_to_f16_sat(v[c][i]);
-          *reinterpret_cast<uint4*>(p.out16 + row * p.ldo + e) = h4;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = tid + (c * 8 + i) * T;
-        if (e < k) {
-          q[e] = (signed char)(rs.bad ? 0 : __float2int_rn(v[c][i] * rs.f));
-          if (KIND == ROW_NORM && p.out16)
-            p.out16[row * p.ldo + e] = rs.bad ? __ushort_as_half(0x7fff) : f32_to_f16_sat(v[c][i]);
-        }
-      }
+    const int e = e0 + c * e_step;
+    const uint2 codes = rs.bad ? make_uint2(0u, 0u) : codes8(v[c], rs.f);
+    if (!VEC) store_codes_shifted(p.q + row * p.ldq, e, k, shift, codes);
+    if (e < k && owner) {
+      if (VEC) *reinterpret_cast<uint2*>(p.q + row * p.ldq + e) = codes;
+      if (KIND == ROW_NORM && p.delta)
+        store8_half<VEC>(x_row + (long long)e * 2, max(0, -e), k - e, make_uint4(xr[c][0], xr[c][1], xr[c][2], xr[c][3]));
+      if (KIND == ROW_NORM && p.out16) store8_half<VEC>(p.out16 + row * p.ldo + e, max(0, -e), k - e, rs.bad ? nan4 : pack_f16_sat(v[c]));
     }
   }
 }
@@ -284,21 +319,25 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
 // Many rows: persistent blocks with a ring of whole rows in shared memory, filled by bulk copies several rows ahead, so
 // the memory system stays busy while a block reduces, quantises and stores. A row's slot is refilled as soon as the
 // reduction's barrier has shown that every thread holds its part in registers: one barrier per row.
-template <int KIND, int MAXC>
-__global__ void __launch_bounds__(MAXC == 4 ? 640 : 1024) row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
+// Rows so wide that an SM holds a single block: TEAMS = 2 halves of the block take turns on the rows of one ring, so one
+// half computes while the other waits for its row or its barrier (4096 x 17408 SwiGLU: 71 -> 57 us).
+template <int KIND, int MAXC, int TEAMS>
+__global__ void __launch_bounds__(TEAMS == 2 ? 1024 : MAXC == 4 ? 640 : 1024, MAXC == 4 && KIND != ROW_NORM ? 2 : 1)
+row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ __align__(8) uint64_t full[RING_SLOTS];
-  __shared__ unsigned red_m[2][32];
-  __shared__ float red_s[2][32];
-  __shared__ int stuck;
+  __shared__ unsigned red_m[TEAMS][2][32];
+  __shared__ float red_s[TEAMS][2][32];
+  __shared__ int stuck[TEAMS];
   constexpr int ES = KIND == ROW_F32 ? 4 : 2;
   pdl_trigger();
-  const int k = p.k, T = blockDim.x, step = gridDim.x;
+  const int k = p.k, T = blockDim.x / TEAMS, step = gridDim.x;
+  const int team = TEAMS == 1 ? 0 : (int)threadIdx.x / T, tid = threadIdx.x - team * T;
   const uint32_t x_bytes = (uint32_t)k * ES * (KIND == ROW_SWIGLU ? 2 : 1);
   const bool two = KIND == ROW_NORM && p.delta;
   if (threadIdx.x == 0) {
     for (int i = 0; i < slots; ++i) mbar_init(full + i, 1);
-    stuck = 0;
+    for (int i = 0; i < TEAMS; ++i) stuck[i] = 0;
     fence_mbar_init();
   }
   __syncthreads();
@@ -311,20 +350,20 @@ __global__ void __launch_bounds__(MAXC == 4 ? 640 : 1024) row_int8_ring_kernel(c
   pdl_wait();
   if (threadIdx.x == 0)
     for (int i = 0; i < slots && (int)blockIdx.x + i * step < n; ++i) fill(i, blockIdx.x + (size_t)i * step);
-  int slot = 0, it = 0;
+  // the block's rows are blockIdx.x + j * step in slots j % slots; a team takes every TEAMS-th of them
+  int slot = team, it = 0;
   uint32_t ph = 0;
-  for (int row = blockIdx.x; row < n; row += step, ++it) {
+  for (long long row = blockIdx.x + (long long)team * step; row < n; row += (long long)TEAMS * step, ++it) {
     if (!mbar_wait(full + slot, ph)) {
       if (p.err) atomicCAS(p.err, 0, (int)VG_ERR_TMA_WAIT);
-      stuck = 1;
+      stuck[team] = 1;
     }
     const uint8_t* src = ring + (size_t)slot * slot_bytes;
     float v[MAXC][8];
-    unsigned mx = 0;
-    float ss = 0.f;
+    float amax = 0.f, ss = 0.f;
 #pragma unroll
     for (int c = 0; c < MAXC; ++c) {
-      const int e = (threadIdx.x + c * T) * 8;
+      const int e = (tid + c * T) * 8;
       if (e < k) {
         if (KIND == ROW_F32) {
           *reinterpret_cast<float4*>(v[c]) = *reinterpret_cast<const float4*>(src + (size_t)e * 4);
@@ -361,16 +400,17 @@ __global__ void __launch_bounds__(MAXC == 4 ? 640 : 1024) row_int8_ring_kernel(c
         for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(v[c][i]) & 0x7fffffffu);
+      for (int i = 0; i < 8; i += 2) amax = max_abs3(amax, v[c][i], v[c][i + 1]);
     }
-    block_reduce<KIND == ROW_NORM>(mx, ss, red_m[it & 1], red_s[it & 1]);
-    if (stuck) break;                                      // seen by every thread: set before the barrier
-    if (threadIdx.x == 0 && row + (long long)slots * step < n) fill(slot, row + (size_t)slots * step);
+    unsigned mx = __float_as_uint(amax);
+    block_reduce<KIND == ROW_NORM>(mx, ss, red_m[team][it & 1], red_s[team][it & 1], tid, T, team + 1);
+    if (stuck[team]) break;                                // seen by the whole team: set before the barrier
+    if (tid == 0 && row + (long long)slots * step < n) fill(slot, row + (size_t)slots * step);
     const RowScale rs = row_scale<KIND>(p, mx, ss);
-    if (threadIdx.x == 0) p.scale[row] = rs.s;
+    if (tid == 0) p.scale[row] = rs.s;
 #pragma unroll
     for (int c = 0; c < MAXC; ++c) {
-      const int e = (threadIdx.x + c * T) * 8;
+      const int e = (tid + c * T) * 8;
       if (e < k) {
         if (KIND == ROW_NORM) {
 #pragma unroll
@@ -383,9 +423,10 @@ __global__ void __launch_bounds__(MAXC == 4 ? 640 : 1024) row_int8_ring_kernel(c
         }
       }
     }
-    if (++slot == slots) { slot = 0; ph ^= 1; }
+    slot += TEAMS;
+    if (slot >= slots) { slot -= slots; ph ^= 1; }
   }
-  if (stuck && threadIdx.x == 0)
+  if (stuck[team] && tid == 0)
     for (int i = 0; i < 64; ++i) __nanosleep(1000);        // let copies in flight land before the block ends
 }
 
@@ -395,51 +436,101 @@ template <> VG_DEVINL float from_f32<float>(float v) { return v; }
 template <> VG_DEVINL __half from_f32<__half>(float v) { return v != v ? __ushort_as_half(0x7fff) : f32_to_f16_sat(v); }
 template <> VG_DEVINL __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight codes per thread where the width and the addresses allow wide accesses, else one.
-template <typename OUT, bool VEC>
-__global__ void __launch_bounds__(256) dequant_int8_kernel(const signed char* __restrict__ q, long long ldq,
-                                                           const float* __restrict__ scale, OUT* __restrict__ out,
-                                                           long long ldo, int k) {
+// Read-back, eight codes per thread and row, R rows per block so that R loads are in flight. (Sixteen per thread leave two
+// 16-byte stores 32 bytes apart per lane: 15.8 us instead of 10.8 at 4096 x 5120.)
+template <typename OUT>
+VG_DEVINL void dequant4(uint32_t c, float s, OUT* o) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = from_f32<OUT>((float)(signed char)(c >> (8 * i)) * s);
+}
+template <typename OUT, int R>
+__global__ void __launch_bounds__(1024) dequant_int8_kernel(const signed char* __restrict__ q, long long ldq,
+                                                            const float* __restrict__ scale, OUT* __restrict__ out,
+                                                            long long ldo, int n, int k) {
+  pdl_trigger();
+  pdl_wait();
+  const long long row0 = (long long)blockIdx.x * R;
+  const int e = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+  if (e >= k) return;
+  uint2 c[R];
+  float s[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (R > 1 && row0 + r >= n) break;
+    c[r] = *reinterpret_cast<const uint2*>(q + (row0 + r) * ldq + e);
+    s[r] = scale[row0 + r];
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (R > 1 && row0 + r >= n) break;
+    alignas(16) OUT o[8];
+    dequant4(c[r].x, s[r], o);
+    dequant4(c[r].y, s[r], o + 4);
+    OUT* dst = out + (row0 + r) * ldo + e;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(OUT) / 2; ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(o)[i];
+  }
+}
+
+// Any width and pitch: groups of eight that start on the output's 16-byte boundaries; their codes come from the two
+// aligned words around them where those lie inside the row.
+template <typename OUT>
+__global__ void __launch_bounds__(256) dequant_int8_loose_kernel(const signed char* __restrict__ q, long long ldq,
+                                                                 const float* __restrict__ scale, OUT* __restrict__ out,
+                                                                 long long ldo, int k) {
   pdl_trigger();
   pdl_wait();
   const size_t row = blockIdx.x;
   const float s = scale[row];
   const signed char* src = q + row * ldq;
   OUT* dst = out + row * ldo;
-  constexpr int W = VEC ? 8 : 1;
-  for (int e = (blockIdx.y * blockDim.x + threadIdx.x) * W; e < k; e += gridDim.y * blockDim.x * W) {
-    if (VEC) {
-      const uint2 c2 = *reinterpret_cast<const uint2*>(src + e);
-      const signed char* c = reinterpret_cast<const signed char*>(&c2);
+  const int head = (int)((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / (int)sizeof(OUT);   // elements before the first boundary
+  for (int g = blockIdx.y * blockDim.x + threadIdx.x;; g += gridDim.y * blockDim.x) {
+    const int e = head + (g - 1) * 8;
+    if (e >= k) break;
+    const uint32_t mis = (uint32_t)(reinterpret_cast<uintptr_t>(src + e) & 7);
+    const signed char* a0 = src + e - (int)mis;
+    if (e >= 0 && e + 8 <= k && (mis == 0 || (a0 >= src && a0 + 16 <= src + k))) {
+      unsigned long long w = *reinterpret_cast<const unsigned long long*>(a0);
+      if (mis) w = (w >> (8 * mis)) | (*reinterpret_cast<const unsigned long long*>(a0 + 8) << (64 - 8 * mis));
       alignas(16) OUT o[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = from_f32<OUT>((float)c[i] * s);
+      dequant4((uint32_t)w, s, o);
+      dequant4((uint32_t)(w >> 32), s, o + 4);
 #pragma unroll
       for (int i = 0; i < (int)sizeof(OUT) / 2; ++i) reinterpret_cast<uint4*>(dst + e)[i] = reinterpret_cast<const uint4*>(o)[i];
     } else {
-      dst[e] = from_f32<OUT>((float)src[e] * s);
+      for (int i = max(0, -e); i < 8 && e + i < k; ++i) dst[e + i] = from_f32<OUT>((float)src[e + i] * s);
     }
   }
 }
 
-constexpr int RING_BYTES = 200 * 1024;            // ring of all blocks of an SM
-constexpr int RING_PER_SM = 4;                    // blocks per SM
-constexpr int RING_MIN_ROWS = 2;                  // rows per SM from which the ring form pays
+// Ring of all blocks of an SM. More of it leaves too little L1 for the norm's weights (4096 x 17408: 86 us with 200 KB, 94
+// with 212); two teams without weights want a third slot.
+constexpr int RING_BYTES = 200 * 1024, RING_TEAM_BYTES = 212 * 1024;
+constexpr int RING_PER_SM = 16;                   // blocks per SM
+constexpr int RING_MIN_ROWS = 8;                  // rows per SM from which the ring form pays
+constexpr int RING_MIN_WIDE = 1;                  // the same for rows of more than 8192
 
-// Largest row width: a cluster of eight CTAs of 1024 threads with two groups of eight each.
+// Largest row width: a cluster of eight CTAs of 1024 threads with two (three) groups of eight each.
 constexpr int ROW_MAX = MAX_CLUSTER * 1024 * 2 * 8;
 
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 template <int KIND, bool VEC>
 cudaError_t launch_shape(RowParams p, int n, cudaStream_t st) {
-  const int groups = (p.k + 7) / 8;
+  // without VEC a row may begin and end inside a group, and a warp has 31 of its own
+  const int groups = VEC ? p.k / 8 : (p.k + 14) / 8, lanes = VEC ? 32 : 31;
+  auto threads = [&](int parts) { return dim3((groups + parts * lanes - 1) / (parts * lanes) * 32); };
   p.cluster = 1;
-  if (groups <= 1024) return launch_pdl(row_int8_kernel<KIND, VEC, 1, false>, dim3(n), dim3((groups + 31) / 32 * 32), 0, st, p);
-  if (groups <= 2048) return launch_pdl(row_int8_kernel<KIND, VEC, 2, false>, dim3(n), dim3((groups + 63) / 64 * 32), 0, st, p);
-  while (p.cluster * 2048 < groups) p.cluster *= 2;
-  const int t = (groups + 2 * p.cluster - 1) / (2 * p.cluster);
-  return launch_pdl_cluster(row_int8_kernel<KIND, VEC, 2, true>, dim3(n * p.cluster), dim3((t + 31) / 32 * 32), p.cluster, 0, st, p);
+  // many shifted rows without a second input: two groups a thread halve the fixed instructions (4096 x 4111 quantise: 25.3
+  // -> 21.3 us; the norm and SwiGLU lose 8 - 20 % to fewer threads)
+  const bool two = !VEC && KIND <= ROW_F32 && n >= 592;
+  if (groups <= 32 * lanes && !two) return launch_pdl(row_int8_kernel<KIND, VEC, 1, false>, dim3(n), threads(1), 0, st, p);
+  if (groups <= 64 * lanes) return launch_pdl(row_int8_kernel<KIND, VEC, 2, false>, dim3(n), threads(2), 0, st, p);
+  while (p.cluster < MAX_CLUSTER && p.cluster * 64 * lanes < groups) p.cluster *= 2;
+  if (VEC || groups <= p.cluster * 64 * lanes)
+    return launch_pdl_cluster(row_int8_kernel<KIND, VEC, 2, true>, dim3(n * p.cluster), threads(2 * p.cluster), p.cluster, 0, st, p);
+  return launch_pdl_cluster(row_int8_kernel<KIND, false, 3, true>, dim3(n * p.cluster), threads(3 * p.cluster), p.cluster, 0, st, p);
 }
 
 int sm_count() {
@@ -451,25 +542,27 @@ int sm_count() {
   return n;
 }
 
-template <int KIND, int MAXC>
+template <int KIND, int MAXC, int TEAMS>
 int launch_ring(const RowParams& p, int n, int slot_bytes, int sms, cudaStream_t st) {
+  constexpr int BYTES = TEAMS == 2 ? RING_TEAM_BYTES : RING_BYTES;
   static std::atomic<unsigned long long> done{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   if (!(done.load() & (1ull << (dev & 63)))) {
-    e = cudaFuncSetAttribute(row_int8_ring_kernel<KIND, MAXC>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES);
+    e = cudaFuncSetAttribute(row_int8_ring_kernel<KIND, MAXC, TEAMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
     if (e != cudaSuccess) return (int)e;
     done.fetch_or(1ull << (dev & 63));
   }
   const int groups = p.k / 8, threads = ((groups + MAXC - 1) / MAXC + 31) / 32 * 32;
-  const int per_sm = max(1, min(min(RING_PER_SM, 1536 / threads), RING_BYTES / (2 * slot_bytes)));
-  const int slots = max(2, min(RING_SLOTS, RING_BYTES / per_sm / slot_bytes));
+  const int room = BYTES / slot_bytes;        // slots an SM holds
+  const int per_sm = TEAMS == 2 ? 1 : max(1, min(min(RING_PER_SM, 2048 / threads), max(room / 3, min(2, room / 2))));
+  const int slots = max(2, min(RING_SLOTS, BYTES / per_sm / slot_bytes));
   const int grid = min(n, sms * per_sm);
-  return (int)launch_pdl(row_int8_ring_kernel<KIND, MAXC>, dim3(grid), dim3(threads), (size_t)slots * slot_bytes, st, p, n, slots, slot_bytes);
+  return (int)launch_pdl(row_int8_ring_kernel<KIND, MAXC, TEAMS>, dim3(grid), dim3(threads * TEAMS), (size_t)slots * slot_bytes, st, p, n, slots, slot_bytes);
 }
 
-// `esize`: bytes of one input element; the wide path wants whole groups of eight and 16-byte addresses on every row
+// `esize`: bytes of one input element; VEC wants whole groups of eight and 16-byte addresses on every row
 template <int KIND>
 int launch_row(const RowParams& p, int n, int esize, cudaStream_t st) {
   if (p.k <= 0 || p.k > ROW_MAX || n < 0 || n > (1 << 27)) return -2;
@@ -481,12 +574,14 @@ int launch_row(const RowParams& p, int n, int esize, cudaStream_t st) {
     if (p.delta) vec = vec && aligned(p.delta, 16) && (n == 1 || p.ldd % 8 == 0);
     if (p.out16) vec = vec && aligned(p.out16, 16) && (n == 1 || p.ldo % 8 == 0);
   }
-  const int sms = sm_count(), slot = p.k * esize * ((KIND == ROW_SWIGLU || p.delta) ? 2 : 1);
-  if (vec && n >= RING_MIN_ROWS * sms && slot % 16 == 0 && 2 * slot <= RING_BYTES && p.k <= 640 * 32) {
-    const int groups = p.k / 8;
-    return groups <= 32 ? launch_ring<KIND, 1>(p, n, slot, sms, st)
-           : groups <= 1024 ? launch_ring<KIND, 2>(p, n, slot, sms, st)
-                            : launch_ring<KIND, 4>(p, n, slot, sms, st);
+  const int sms = sm_count(), slot = p.k * esize * ((KIND == ROW_SWIGLU || p.delta) ? 2 : 1), groups = p.k / 8;
+  if (vec && n >= (groups > 1024 ? RING_MIN_WIDE : RING_MIN_ROWS) * sms && slot % 16 == 0 && 2 * slot <= RING_BYTES && groups <= 2560) {
+    if constexpr (KIND == ROW_SWIGLU) {
+      if (4 * slot > RING_BYTES && groups > 1024) return launch_ring<KIND, 5, 2>(p, n, slot, sms, st);
+    }
+    return groups <= 32 ? launch_ring<KIND, 1, 1>(p, n, slot, sms, st)
+           : groups <= 1024 ? launch_ring<KIND, 2, 1>(p, n, slot, sms, st)
+                            : launch_ring<KIND, 4, 1>(p, n, slot, sms, st);
   }
   const cudaError_t e = vec ? launch_shape<KIND, true>(p, n, st) : launch_shape<KIND, false>(p, n, st);
   return (int)e;
@@ -496,11 +591,13 @@ template <typename OUT>
 int launch_dequant(const signed char* q, long long ldq, const float* scale, void* out, long long ldo, int n, int k,
                    cudaStream_t st) {
   const bool vec = k % 8 == 0 && aligned(q, 8) && aligned(out, 16) && (n == 1 || (ldq % 8 == 0 && (ldo * sizeof(OUT)) % 16 == 0));
-  const int per = 256 * (vec ? 8 : 1);
-  const dim3 grid(n, min((k + per - 1) / per, 64));
   OUT* o = static_cast<OUT*>(out);
-  return (int)(vec ? launch_pdl(dequant_int8_kernel<OUT, true>, grid, dim3(256), 0, st, q, ldq, scale, o, ldo, k)
-                   : launch_pdl(dequant_int8_kernel<OUT, false>, grid, dim3(256), 0, st, q, ldq, scale, o, ldo, k));
+  if (!vec)
+    return (int)launch_pdl(dequant_int8_loose_kernel<OUT>, dim3(n, min((k / 8 + 2 + 255) / 256, 64)), dim3(256), 0, st, q, ldq, scale,
+                           o, ldo, k);
+  const int words = k / 8, ny = (words + 1023) / 1024, threads = ((words + ny - 1) / ny + 31) / 32 * 32;
+  if (n >= 512) return (int)launch_pdl(dequant_int8_kernel<OUT, 4>, dim3((n + 3) / 4, ny), dim3(threads), 0, st, q, ldq, scale, o, ldo, n, k);
+  return (int)launch_pdl(dequant_int8_kernel<OUT, 1>, dim3(n, ny), dim3(threads), 0, st, q, ldq, scale, o, ldo, n, k);
 }
 }  // namespace
 

@@ -108,6 +108,83 @@ def test_rows_with_strides_and_spare_rows():
         assert (back[3:] == 5).all() and (back[:, :2] == 5).all() and (back[:, 2 + k:] == 5).all()
 
 
+@pytest.mark.parametrize("off", range(8))
+@pytest.mark.parametrize("k", [1, 5, 9, 24, 250, 263, 4111, 16391])
+def test_rows_at_every_offset(off, k):
+    """Rows and codes that start anywhere: every distance from a 16-byte boundary, for the input, the residual that is written
+    back, the codes and the f16 copy, with nothing touched next to them."""
+    from velogb10_b200.ops import int8 as I8
+    n, pitch = 5, k + off + 3
+    for dtype in (BF, F16, F32):
+        x = _randn((n, pitch), k + off, dtype)[:, off:off + k]
+        q = torch.full((n, pitch), 77, dtype=torch.int8, device="cuda")
+        act = I8.quantize_act_int8(x, out=I8.Int8Act(q[:, off // 2:off // 2 + k], torch.empty(n, device="cuda")))
+        _check_rows(act, x.double(), n, 0.0, (off, k, dtype))
+        assert (q[:, :off // 2] == 77).all() and (q[:, off // 2 + k:] == 77).all()
+        assert torch.equal(I8.quantize_act_int8(x.contiguous()).q, act.q)
+    res = _randn((n, pitch), off, BF)
+    delta, w = _randn((n, k + 1), off + 9, BF)[:, 1:], _randn((k + off,), off)[off:] * 0.1
+    keep, out16 = res.clone(), torch.full((n, pitch), 5.0, dtype=F16, device="cuda")
+    act = I8.add_rmsnorm_int8(res[:, off:off + k], delta, w, 1e-6, out16=out16[:, 2:2 + k])
+    x = (keep[:, off:off + k].double() + delta.double()).to(BF)
+    assert torch.equal(res[:, off:off + k], x)
+    assert torch.equal(res[:, :off], keep[:, :off]) and torch.equal(res[:, off + k:], keep[:, off + k:])
+    y = x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + 1e-6) * (1 + w.double())
+    _check_rows(act, y, n, 27 * 2.0 ** -24, (off, k))
+    assert ((out16[:, 2:2 + k].double() - y).abs() <= y.abs() * (2.0 ** -11 + 27 * 2.0 ** -24) + 2.0 ** -24).all()
+    assert (out16[:, :2] == 5).all() and (out16[:, 2 + k:] == 5).all()
+    gu = _randn((n, 2 * k + off), off + 3, BF)[:, off:]
+    g, u = gu[:, :k].double(), gu[:, k:].double()
+    _check_rows(I8.swiglu_int8(gu), g * torch.sigmoid(g) * u, n, 30 * 2.0 ** -23, (off, k))
+    for dtype in (BF, F16, F32):
+        out = torch.full((n, pitch), 3.0, dtype=dtype, device="cuda")
+        I8.dequantize_act_int8(act, out=out[:, off:off + k])
+        assert torch.equal(out[:, off:off + k], I8.dequantize_act_int8(act, dtype=dtype))
+        assert torch.equal(out[:, off:off + k], (act.q.float() * act.scale[:, None]).to(dtype))
+        assert (out[:, :off] == 3).all() and (out[:, off + k:] == 3).all()
+
+
+# rows enough for the ring of whole rows: several blocks an SM, two, one, and one of two halves; with and without a tail
+@pytest.mark.parametrize("n,k", [(1184, 8), (1300, 512), (2777, 2048), (1200, 5120), (150, 8200), (333, 17408), (149, 20480), (301, 12800)])
+def test_many_rows(n, k):
+    from velogb10_b200.ops import int8 as I8
+    spare = 3
+    for dtype in (BF, F16, F32):
+        x = _randn((n + spare, k), k, dtype)
+        out = I8.act_buffers(n + spare, k, "cuda")
+        out.q.fill_(99)
+        I8.quantize_act_int8(x, n=n, out=out)
+        _check_rows(out, x[:n].double(), n, 0.0, (n, k, dtype))
+        assert (out.q[n:] == 99).all()
+        for r in (0, n // 2, n - 1):                         # a row's bits do not depend on the form
+            one = I8.quantize_act_int8(x[r:r + 1])
+            assert torch.equal(one.q[0], out.q[r]) and torch.equal(one.scale[0], out.scale[r])
+    gu = (_randn((n + spare, 2 * k), k + 1) * 3).to(BF)
+    act = I8.swiglu_int8(gu, n=n)
+    g, u = gu[:n, :k].double(), gu[:n, k:].double()
+    _check_rows(act, g * torch.sigmoid(g) * u, n, 30 * 2.0 ** -23, (n, k))
+    res, delta, w = _randn((n + spare, k), 3, BF), _randn((n + spare, k), 4, BF), _randn((k,), 5) * 0.2
+    for d in (delta, None):
+        x = res.clone()
+        want = (res.double() + d.double()).to(BF) if d is not None else res
+        out16 = torch.empty((n, k), dtype=F16, device="cuda") if d is not None else None
+        act = I8.add_rmsnorm_int8(x, d, w, 1e-6, n=n, out16=out16)
+        y = want[:n].double()
+        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + 1e-6) * (1 + w.double())
+        # per thread at most 40 terms, then 10 shuffles: 51 roundings halved, and 9 more
+        rel = (51 / 2 + 9) * 2.0 ** -24
+        _check_rows(act, y, n, rel, (n, k))
+        assert torch.equal(x[:n], want[:n]) and torch.equal(x[n:], res[n:])
+        if out16 is not None:
+            assert ((out16.double() - y).abs() <= y.abs() * (2.0 ** -11 + rel) + 2.0 ** -24).all()
+    x = _randn((n, k), 6, BF)
+    x[n // 3] = float("nan")
+    x[n - 1] = 0
+    act = I8.quantize_act_int8(x)
+    assert act.scale[n // 3].isnan() and (act.q[n // 3] == 0).all() and float(act.scale[n - 1]) == FLOOR
+    assert act.scale.isnan().sum() == 1
+
+
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("k", [1, 8, 33, 4096, 131071])
 def test_read_back(dtype, k):
