@@ -320,7 +320,10 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
 // the memory system stays busy while a block reduces, quantises and stores. A row's slot is refilled as soon as the
 // reduction's barrier has shown that every thread holds its part in registers: one barrier per row.
 // Rows so wide that an SM holds a single block: TEAMS = 2 halves of the block take turns on the rows of one ring, so one
-// half computes while the other waits for its row or its barrier (4096 x 17408 SwiGLU: 71 -> 57 us).
+// half computes while the other waits for its row or its barrier (4096 x 17408 SwiGLU: 71 -> 57 us). A slot of an odd ring
+// passes from one team to the other, so a team may come to a slot whose previous row has not even landed (copies may land
+// out of order); the one-bit parity of its barrier cannot tell that phase from the one waited for. `filled` can: it names
+// the row whose copy was last issued into the slot, and a team looks at the barrier only once its own row is there.
 template <int KIND, int MAXC, int TEAMS>
 __global__ void __launch_bounds__(TEAMS == 2 ? 1024 : MAXC == 4 ? 640 : 1024, MAXC == 4 && KIND != ROW_NORM ? 2 : 1)
 row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
@@ -329,6 +332,7 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
   __shared__ unsigned red_m[TEAMS][2][32];
   __shared__ float red_s[TEAMS][2][32];
   __shared__ int stuck[TEAMS];
+  __shared__ volatile int filled[RING_SLOTS];
   constexpr int ES = KIND == ROW_F32 ? 4 : 2;
   pdl_trigger();
   const int k = p.k, T = blockDim.x / TEAMS, step = gridDim.x;
@@ -336,25 +340,39 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
   const uint32_t x_bytes = (uint32_t)k * ES * (KIND == ROW_SWIGLU ? 2 : 1);
   const bool two = KIND == ROW_NORM && p.delta;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < slots; ++i) mbar_init(full + i, 1);
+    for (int i = 0; i < slots; ++i) {
+      mbar_init(full + i, 1);
+      filled[i] = -1;
+    }
     for (int i = 0; i < TEAMS; ++i) stuck[i] = 0;
     fence_mbar_init();
   }
   __syncthreads();
-  auto fill = [&](int slot, size_t row) {
+  auto fill = [&](int slot, int j, size_t row) {
     uint8_t* dst = ring + (size_t)slot * slot_bytes;
     mbar_arrive_expect_tx(full + slot, two ? 2 * x_bytes : x_bytes);
     tma_bulk_g2s(dst, static_cast<const char*>(p.x) + row * p.ldx * ES, x_bytes, full + slot);
     if (two) tma_bulk_g2s(dst + x_bytes, p.delta + row * p.ldd, x_bytes, full + slot);
+    if (TEAMS > 1) {
+      __threadfence_block();
+      filled[slot] = j;
+    }
   };
   pdl_wait();
   if (threadIdx.x == 0)
-    for (int i = 0; i < slots && (int)blockIdx.x + i * step < n; ++i) fill(i, blockIdx.x + (size_t)i * step);
+    for (int i = 0; i < slots && (int)blockIdx.x + i * step < n; ++i) fill(i, i, blockIdx.x + (size_t)i * step);
   // the block's rows are blockIdx.x + j * step in slots j % slots; a team takes every TEAMS-th of them
   int slot = team, it = 0;
   uint32_t ph = 0;
   for (long long row = blockIdx.x + (long long)team * step; row < n; row += (long long)TEAMS * step, ++it) {
-    if (!mbar_wait(full + slot, ph)) {
+    const int j = it * TEAMS + team;
+    bool ok = true;
+    if (TEAMS > 1) {
+      const uint64_t t0 = global_ns();
+      while (filled[slot] != j && ok) ok = global_ns() - t0 < 200ull * 1000 * 1000;
+      __threadfence_block();
+    }
+    if (!ok || !mbar_wait(full + slot, ph)) {
       if (p.err) atomicCAS(p.err, 0, (int)VG_ERR_TMA_WAIT);
       stuck[team] = 1;
     }
@@ -405,7 +423,7 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
     unsigned mx = __float_as_uint(amax);
     block_reduce<KIND == ROW_NORM>(mx, ss, red_m[team][it & 1], red_s[team][it & 1], tid, T, team + 1);
     if (stuck[team]) break;                                // seen by the whole team: set before the barrier
-    if (tid == 0 && row + (long long)slots * step < n) fill(slot, row + (size_t)slots * step);
+    if (tid == 0 && row + (long long)slots * step < n) fill(slot, j + slots, row + (size_t)slots * step);
     const RowScale rs = row_scale<KIND>(p, mx, ss);
     if (tid == 0) p.scale[row] = rs.s;
 #pragma unroll

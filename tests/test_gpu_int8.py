@@ -185,6 +185,29 @@ def test_many_rows(n, k):
     assert act.scale.isnan().sum() == 1
 
 
+def test_wide_rows_under_load():
+    """Two halves of a block share a ring of three rows whose copies may land in any order: the same bits every time, with
+    other kernels (on another stream, and the read-back right behind) competing for memory."""
+    from velogb10_b200.ops import int8 as I8, lib
+    n, k = 4096, 17408
+    gu = torch.randn((n, 2 * k), generator=_gen(0), device="cuda").to(BF)
+    want = I8.swiglu_int8(gu)
+    for r in (0, 1, 147, 148, 149, 1000, n - 1):
+        one = I8.swiglu_int8(gu[r:r + 1])
+        assert torch.equal(one.q[0], want.q[r]) and torch.equal(one.scale[0], want.scale[r])
+    side, noise = torch.cuda.Stream(), torch.empty_like(gu)
+    for i in range(20):
+        if i % 2:
+            with torch.cuda.stream(side):
+                noise.copy_(gu)
+        act = I8.swiglu_int8(gu)
+        back = I8.dequantize_act_int8(act)
+        assert torch.equal(act.q, want.q) and torch.equal(act.scale, want.scale)
+        assert back.isfinite().all()
+    torch.cuda.synchronize()
+    lib.check_err_word()
+
+
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("k", [1, 8, 33, 4096, 131071])
 def test_read_back(dtype, k):

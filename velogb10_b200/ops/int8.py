@@ -24,6 +24,7 @@ from .lib import KernelError, c_float, c_int, c_ll, c_void_p
 MAX_K = 131071                 # 128 * 128 * K must stay below 2^31
 MAX_ROWS = 1 << 27
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_BF16, _INT8 = (torch.bfloat16,), (torch.int8,)
 
 
 @dataclass
@@ -36,8 +37,8 @@ class Int8Act:
 def act_buffers(rows: int, k: int, device) -> Int8Act:
     """Buffers a quantiser can write into (``out=``) and ``linear_int8`` can read."""
     kp = (k + 15) & ~15
-    q = torch.empty((rows, kp), dtype=torch.int8, device=device)
-    return Int8Act(q if kp == k else q[:, :k], torch.empty((rows,), dtype=torch.float32, device=device))
+    q = torch.empty(rows, kp, dtype=torch.int8, device=device)
+    return Int8Act(q if kp == k else q[:, :k], torch.empty(rows, dtype=torch.float32, device=device))
 
 
 _fns = {}
@@ -71,19 +72,28 @@ def _launch(name: str, device: torch.device, *args):
         _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name)
 
 
+_err_ptrs = {}
+
+
 def _err(device: torch.device) -> int:
-    return _lib.err_word(device).data_ptr() if device.type == "cuda" else 0
+    p = _err_ptrs.get(device)
+    if p is None:
+        if device.type != "cuda":
+            return 0                                    # refused by _launch
+        p = _err_ptrs[device] = _lib.err_word(device).data_ptr()
+    return p
 
 
-def _rows(t: torch.Tensor, n: Optional[int], what: str) -> int:
+def _input(t: torch.Tensor, what: str, dtypes, n: Optional[int]):
+    """Rows to process, row width and row pitch of a call's main argument."""
     if t.dim() != 2:
         raise KernelError(f"{what}: expected a matrix, got shape {tuple(t.shape)}")
-    rows = t.shape[0]
+    rows, cols = t.shape
     if n is None:
         n = rows
     if not 0 <= n <= rows or n > MAX_ROWS:
         raise KernelError(f"{what}: {n} rows asked for, the tensor has {rows}")
-    return n
+    return n, cols, _matrix(t, what, dtypes, n, cols)
 
 
 def _matrix(t: torch.Tensor, what: str, dtypes, rows: int, cols: int, device=None) -> int:
@@ -113,17 +123,16 @@ def _out(out: Optional[Int8Act], n: int, k: int, device):
         raise KernelError(f"row width {k} is outside 1 .. {MAX_K}")
     if out is None:
         return act_buffers(n, k, device), (k + 15) & ~15
-    ld = _matrix(out.q, "out.q", (torch.int8,), n, k, device)
+    ld = _matrix(out.q, "out.q", _INT8, n, k, device)
     _vector(out.scale, "out.scale", n, device, least=True)
     return out, ld
 
 
 def quantize_act_int8(x: torch.Tensor, n: Optional[int] = None, out: Optional[Int8Act] = None) -> Int8Act:
     """Quantise rows ``x[:n]`` (bf16 / f16 / f32 ``[rows, k]``)."""
-    n = _rows(x, n, "x")
-    k, dev = x.shape[1], x.device
+    n, k, ld = _input(x, "x", _DTYPE, n)
+    dev = x.device
     out, ldq = _out(out, n, k, dev)
-    ld = _matrix(x, "x", _DTYPE, n, k)
     if n:
         _launch("vg_quant_int8", dev, x.data_ptr(), ld, _DTYPE[x.dtype], n, k, out.q.data_ptr(), ldq, out.scale.data_ptr(), _err(dev))
     return out
@@ -131,13 +140,15 @@ def quantize_act_int8(x: torch.Tensor, n: Optional[int] = None, out: Optional[In
 
 def swiglu_int8(gu: torch.Tensor, n: Optional[int] = None, inter: Optional[int] = None, out: Optional[Int8Act] = None) -> Int8Act:
     """``silu(gate) * up`` of ``gu[:n] = [gate | up]`` (bf16 ``[rows, 2 * inter]``), quantised."""
-    n = _rows(gu, n, "gu")
+    n, cols, ld = _input(gu, "gu", _BF16, n)
     if inter is None:
-        inter = gu.shape[1] // 2
-    ld = _matrix(gu, "gu", (torch.bfloat16,), n, 2 * inter)
-    out, ldq = _out(out, n, inter, gu.device)
+        inter = cols // 2
+    if cols != 2 * inter:
+        raise KernelError(f"gu: {cols} columns, expected 2 * {inter}")
+    dev = gu.device
+    out, ldq = _out(out, n, inter, dev)
     if n:
-        _launch("vg_swiglu_int8", gu.device, gu.data_ptr(), ld, n, inter, out.q.data_ptr(), ldq, out.scale.data_ptr(), _err(gu.device))
+        _launch("vg_swiglu_int8", dev, gu.data_ptr(), ld, n, inter, out.q.data_ptr(), ldq, out.scale.data_ptr(), _err(dev))
     return out
 
 
@@ -145,15 +156,14 @@ def add_rmsnorm_int8(res: torch.Tensor, delta: Optional[torch.Tensor], w: torch.
                      out: Optional[Int8Act] = None, out16: Optional[torch.Tensor] = None, plus_one: bool = True) -> Int8Act:
     """``res[:n] += delta[:n]`` (bf16, in place, when delta is given), then RMSNorm with weights ``w`` (``1 + w`` with
     ``plus_one``) quantised; the normed rows also go to ``out16`` (f16, saturating) when it is given."""
-    n = _rows(res, n, "res")
-    h, dev = res.shape[1], res.device
+    n, h, ld = _input(res, "res", _BF16, n)
+    dev = res.device
     if not eps > 0.0:
         raise KernelError(f"eps must be positive, got {eps}")
     out, ldq = _out(out, n, h, dev)
-    ld = _matrix(res, "res", (torch.bfloat16,), n, h)
     ldd = ldo = 0
     if delta is not None:
-        ldd = _matrix(delta, "delta", (torch.bfloat16,), n, h, dev)
+        ldd = _matrix(delta, "delta", _BF16, n, h, dev)
     if out16 is not None:
         ldo = _matrix(out16, "out16", (torch.float16,), n, h, dev)
     _vector(w, "w", h, dev)
@@ -167,17 +177,18 @@ def add_rmsnorm_int8(res: torch.Tensor, delta: Optional[torch.Tensor], w: torch.
 def dequantize_act_int8(act: Int8Act, n: Optional[int] = None, out: Optional[torch.Tensor] = None,
                         dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values rows ``act.q[:n]`` stand for, in bf16, f16 (saturating) or f32 (``out``'s type when it is given)."""
-    n = _rows(act.q, n, "act.q")
-    k, dev = act.q.shape[1], act.q.device
+    n, k, ldq = _input(act.q, "act.q", _INT8, n)
+    dev = act.q.device
     if k < 1 or k > MAX_K:
         raise KernelError(f"row width {k} is outside 1 .. {MAX_K}")
-    ldq = _matrix(act.q, "act.q", (torch.int8,), n, k)
     _vector(act.scale, "act.scale", n, dev, least=True)
     if out is None:
         if dtype not in _DTYPE:
             raise KernelError(f"dtype {dtype} is not supported")
-        out = torch.empty((n, k), dtype=dtype, device=dev)
-    ldo = _matrix(out, "out", _DTYPE, n, k, dev)
+        out = torch.empty(n, k, dtype=dtype, device=dev)
+        ldo = k
+    else:
+        ldo = _matrix(out, "out", _DTYPE, n, k, dev)
     if n:
         _launch("vg_dequant_int8", dev, act.q.data_ptr(), ldq, act.scale.data_ptr(), out.data_ptr(), ldo, _DTYPE[out.dtype], n, k)
     return out
@@ -189,12 +200,13 @@ def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional
     read in place: rows must start on 16-byte boundaries (``codec.rows16`` re-lays a matrix whose rows do not)."""
     if q.fmt != "int8":
         raise KernelError(f"linear_int8 takes int8 weights, got {q.fmt}")
-    n = _rows(act.q, n, "act.q")
+    n, cols, ldq = _input(act.q, "act.q", _INT8, n)
     m, k, dev = q.m, q.k, act.q.device
     if k < 1 or k > MAX_K or m < 1:
         raise KernelError(f"weights [{m}, {k}]: K must be in 1 .. {MAX_K}")
-    ldw = _matrix(q.codes, "codes", (torch.int8,), m, k, dev)
-    ldq = _matrix(act.q, "act.q", (torch.int8,), n, k)
+    if cols != k:
+        raise KernelError(f"act.q: {cols} columns, the weights have {k}")
+    ldw = _matrix(q.codes, "codes", _INT8, m, k, dev)
     if m == 1:
         ldw = (k + 15) & ~15
     if n <= 1:
@@ -205,7 +217,7 @@ def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional
     _vector(q.row_scale, "row_scale", m, dev)
     _vector(act.scale, "act.scale", n, dev, least=True)
     if out is None:
-        out = torch.empty((n, m), dtype=torch.float32 if out_f32 else torch.bfloat16, device=dev)
+        out = torch.empty(n, m, dtype=torch.float32 if out_f32 else torch.bfloat16, device=dev)
         ldo = m
     else:
         ldo = _matrix(out, "out", (torch.bfloat16, torch.float32), n, m, dev)
