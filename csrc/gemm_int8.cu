@@ -10,8 +10,8 @@
 // K of both arrive by tiled TMA with the 128-byte swizzle (zeros beyond K, the channels and the tokens). Two forms:
 //   narrow  up to 64 tokens: one CTA per 128 channels, bound by the weight stream
 //   pair    more: a pair of CTAs per 256 channels x up to 256 tokens (cta_group::2), bound by the MMAs
-// Both have 192 threads: warp 0 copies, warp 1 issues four K = 32 MMAs per slab, warps 2-5 read the accumulator back,
-// thread = output channel. With few tiles K is split over a cluster and the partial sums meet in distributed shared
+// In both warp 0 copies, warp 1 issues four K = 32 MMAs per slab, and four or eight more warps read the accumulator back,
+// lane = output channel. With few tiles K is split over a cluster and the partial sums meet in distributed shared
 // memory. All waits are bounded.
 #include <cuda.h>
 #include <atomic>
@@ -28,6 +28,8 @@ constexpr int BK = 128;                     // bytes of K per slab
 constexpr int A_BYTES = BM * BK;
 constexpr int THREADS = 192;
 constexpr int MAX_SPLIT = 8;
+constexpr int NARROW_MAX = 64;              // tokens of the narrow form
+constexpr int SX_PAD = 4;                   // read past a tile's last token scale, never used
 
 struct I8Params {
   const float* sx;
@@ -87,43 +89,94 @@ struct OutWarp {
   }
 };
 
-// Stores columns [c, c + 4) (`v`, int32 sums of this lane's channel), `left` of which hold a token. A warp has 32
-// channels of one token per register, so storing registers as they are takes one 2-byte store per value and lane: 50
-// cycles a column, 13 k cycles for a 256-column tile against 20 k of MMAs at K = 5120. The vec form transposes 4 x 4
-// blocks among neighbouring lanes first (two shuffles), then each lane stores four channels of one token.
-VG_DEVINL void store4(const I8Params& p, const OutWarp& o, int c, const uint32_t* v, const float4 sx, int left) {
-  const float y0 = (float)(int)v[0] * o.sw * sx.x, y1 = (float)(int)v[1] * o.sw * sx.y;
-  const float y2 = (float)(int)v[2] * o.sw * sx.z, y3 = (float)(int)v[3] * o.sw * sx.w;
-  if (!p.vec) {
-    const float y[4] = {y0, y1, y2, y3};
+// Stores G groups of four columns (`v`, int32 sums of this lane's channel). Group g is columns c[g] .. c[g] + 3, of which
+// those below `cols` hold a token; `sx` has the tile's token scales.
+// A warp has 32 channels of one token per register, so storing registers as they are takes one 2-byte store per value and
+// lane. The vec form transposes 4 x 4 blocks among neighbouring lanes first (two or four shuffles), then each lane stores
+// four channels of one token. A scheduler has one or two of these warps, so what counts is that all groups' chains are
+// independent and in one basic block: with a branch per group a 256-column tile took 11.4 k cycles, this way EPI_NOTE.
+template <bool F32, bool VEC, int G>
+VG_DEVINL void store_groups(const OutWarp& o, const int* c, int cols, const uint32_t* v, const float* sx) {
+  const int lane = threadIdx.x & 31;
+  const bool b0 = lane & 1, b1 = lane & 2;
+  float y[G][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (o.in && i < left) {
-        char* d = o.base + (size_t)(c + i) * o.pitch;
-        if (p.out_f32) *reinterpret_cast<float*>(d) = y[i];
-        else *reinterpret_cast<__nv_bfloat16*>(d) = __float2bfloat16_rn(y[i]);
+  for (int g = 0; g < G; ++g) {
+    const float4 s = *reinterpret_cast<const float4*>(sx + c[g]);
+    y[g][0] = (float)(int)v[4 * g] * o.sw * s.x;
+    y[g][1] = (float)(int)v[4 * g + 1] * o.sw * s.y;
+    y[g][2] = (float)(int)v[4 * g + 2] * o.sw * s.z;
+    y[g][3] = (float)(int)v[4 * g + 3] * o.sw * s.w;
+  }
+  if (!VEC) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        char* d = o.base + (size_t)(c[g] + i) * o.pitch;
+        if (o.in && c[g] + i < cols) {
+          if (F32) *reinterpret_cast<float*>(d) = y[g][i];
+          else *reinterpret_cast<__nv_bfloat16*>(d) = __float2bfloat16_rn(y[g][i]);
+        }
       }
-    }
     return;
   }
-  const bool b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
-  char* d = o.base + (size_t)c * o.pitch;
-  const bool st = o.in && (int)(threadIdx.x & 3) < left;
-  if (p.out_f32) {
-    const float ra = __shfl_xor_sync(0xffffffffu, b0 ? y0 : y1, 1), rb = __shfl_xor_sync(0xffffffffu, b0 ? y2 : y3, 1);
-    const float2 A = b0 ? make_float2(ra, y1) : make_float2(y0, ra);      // token b0, channels (even, odd)
-    const float2 B = b0 ? make_float2(rb, y3) : make_float2(y2, rb);      // token 2 + b0
-    const float2 snd = b1 ? A : B, own = b1 ? B : A;
-    const float2 rcv = make_float2(__shfl_xor_sync(0xffffffffu, snd.x, 2), __shfl_xor_sync(0xffffffffu, snd.y, 2));
-    if (st) *reinterpret_cast<float4*>(d) = b1 ? make_float4(rcv.x, rcv.y, own.x, own.y) : make_float4(own.x, own.y, rcv.x, rcv.y);
+  if (F32) {
+    float2 A[G], B[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float ra = __shfl_xor_sync(0xffffffffu, b0 ? y[g][0] : y[g][1], 1), rb = __shfl_xor_sync(0xffffffffu, b0 ? y[g][2] : y[g][3], 1);
+      A[g] = b0 ? make_float2(ra, y[g][1]) : make_float2(y[g][0], ra);      // token b0, channels (even, odd)
+      B[g] = b0 ? make_float2(rb, y[g][3]) : make_float2(y[g][2], rb);      // token 2 + b0
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float2 snd = b1 ? A[g] : B[g], own = b1 ? B[g] : A[g];
+      const float2 rcv = make_float2(__shfl_xor_sync(0xffffffffu, snd.x, 2), __shfl_xor_sync(0xffffffffu, snd.y, 2));
+      const float4 w = b1 ? make_float4(rcv.x, rcv.y, own.x, own.y) : make_float4(own.x, own.y, rcv.x, rcv.y);
+      if (o.in && c[g] + (lane & 3) < cols) *reinterpret_cast<float4*>(o.base + (size_t)c[g] * o.pitch) = w;
+    }
   } else {
-    const __nv_bfloat162 e2 = __floats2bfloat162_rn(y0, y2), o2 = __floats2bfloat162_rn(y1, y3);
-    const uint32_t e = *reinterpret_cast<const uint32_t*>(&e2), q = *reinterpret_cast<const uint32_t*>(&o2);
-    const uint32_t own = b0 ? q : e, rcv = __shfl_xor_sync(0xffffffffu, b0 ? e : q, 1);
-    const uint32_t lo = b0 ? rcv : own, hi = b0 ? own : rcv;              // even channel, odd channel
-    const uint32_t w0 = __byte_perm(lo, hi, 0x5410), w1 = __byte_perm(lo, hi, 0x7632);   // tokens b0 and 2 + b0
-    const uint32_t mine = b1 ? w1 : w0, other = __shfl_xor_sync(0xffffffffu, b1 ? w0 : w1, 2);
-    if (st) *reinterpret_cast<uint2*>(d) = b1 ? make_uint2(other, mine) : make_uint2(mine, other);
+    uint32_t w0[G], w1[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const __nv_bfloat162 e2 = __floats2bfloat162_rn(y[g][0], y[g][2]), o2 = __floats2bfloat162_rn(y[g][1], y[g][3]);
+      const uint32_t e = *reinterpret_cast<const uint32_t*>(&e2), q = *reinterpret_cast<const uint32_t*>(&o2);
+      const uint32_t own = b0 ? q : e, rcv = __shfl_xor_sync(0xffffffffu, b0 ? e : q, 1);
+      const uint32_t lo = b0 ? rcv : own, hi = b0 ? own : rcv;              // even channel, odd channel
+      w0[g] = __byte_perm(lo, hi, 0x5410);                                  // tokens b0 and 2 + b0
+      w1[g] = __byte_perm(lo, hi, 0x7632);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint32_t mine = b1 ? w1[g] : w0[g], other = __shfl_xor_sync(0xffffffffu, b1 ? w0[g] : w1[g], 2);
+      const uint2 w = b1 ? make_uint2(other, mine) : make_uint2(mine, other);
+      if (o.in && c[g] + (lane & 3) < cols) *reinterpret_cast<uint2*>(o.base + (size_t)c[g] * o.pitch) = w;
+    }
+  }
+}
+template <int G>
+VG_DEVINL void store_columns(const I8Params& p, const OutWarp& o, const int* c, int cols, const uint32_t* v, const float* sx) {
+  if (p.vec) {
+    if (p.out_f32) store_groups<true, true, G>(o, c, cols, v, sx);
+    else store_groups<false, true, G>(o, c, cols, v, sx);
+  } else {
+    if (p.out_f32) store_groups<true, false, G>(o, c, cols, v, sx);
+    else store_groups<false, false, G>(o, c, cols, v, sx);
+  }
+}
+// Accumulator columns [0, cols) of a whole tile, 4 * G at a time; `of` warps with the same channels take turns.
+template <int G>
+VG_DEVINL void store_tile(const I8Params& p, const OutWarp& o, uint32_t acc, int cols, const float* sx, int turn, int of) {
+  for (int c0 = turn * 4 * G; c0 < cols; c0 += of * 4 * G) {
+    uint32_t v[4 * G];
+#pragma unroll
+    for (int i = 0; i < G / 2; ++i) tmem_ld8(acc + c0 + 8 * i, v + 8 * i);
+    tmem_ld_wait();
+    int c[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) c[g] = c0 + 4 * g;
+    store_columns<G>(p, o, c, cols, v, sx);
   }
 }
 // A warp's own copy of the token scales, fetched while the accumulator is still being built.
@@ -138,17 +191,17 @@ VG_DEVINL void fetch_sx(const I8Params& p, float* sx, int n0, int cols) {
 VG_DEVINL uint32_t group_slots(int cols, int parts) { return (uint32_t)(((cols + 3) / 4 + parts - 1) / parts); }
 // `to_rank(part)`: cluster rank of the CTA of that part which holds the same channels
 template <typename F>
-VG_DEVINL void send_partials(uint32_t area, uint32_t acc, bool have, int cols, int part, int parts, int r, F to_rank) {
+VG_DEVINL void send_partials(uint32_t area, uint32_t acc, bool have, int cols, int part, int parts, int r, int turn, int of, F to_rank) {
   const uint32_t slots = group_slots(cols, parts);
-  int dst = 0;
-  uint32_t slot = 0;
-  for (int c = 0; c < cols; c += 16) {
+  for (int c = turn * 16; c < cols; c += of * 16) {
     uint32_t v[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     if (have) {
       tmem_ld8(acc + c, v);
       if (c + 8 < cols) tmem_ld8(acc + c + 8, v + 8);
       tmem_ld_wait();
     }
+    uint32_t slot = (uint32_t)(c / 4) / (uint32_t)parts;
+    int dst = c / 4 - (int)slot * parts;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (c + 4 * i < cols) dsmem_st_v4(dsmem_map(area + ((part * slots + slot) * BM + r) * 16, to_rank(dst)), v + 4 * i);
@@ -156,19 +209,28 @@ VG_DEVINL void send_partials(uint32_t area, uint32_t acc, bool have, int cols, i
     }
   }
 }
+template <int G>
 VG_DEVINL void finish_partials(const I8Params& p, const uint8_t* area, const OutWarp& o, const float* sx, int cols, int part, int parts,
-                               int r) {
-  const uint32_t slots = group_slots(cols, parts);
+                               int r, int turn, int of) {
+  const int slots = (int)group_slots(cols, parts);
   const uint4* a = reinterpret_cast<const uint4*>(area) + r;
-  for (uint32_t s = 0; s < slots; ++s) {
-    const int c = ((int)s * parts + part) * 4;
-    if (c >= cols) break;
-    uint32_t v[4] = {0, 0, 0, 0};
-    for (int q = 0; q < parts; ++q) {
-      const uint4 w = a[(q * slots + s) * BM];
-      v[0] += w.x; v[1] += w.y; v[2] += w.z; v[3] += w.w;
+  for (int s0 = turn * G; s0 < slots && (s0 * parts + part) * 4 < cols; s0 += of * G) {
+    uint32_t v[4 * G] = {};
+    int c[G];
+    const uint4* at[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      // groups past the end come out as columns from the first multiple of four after `cols` on, which are not stored
+      c[g] = min(((s0 + g) * parts + part) * 4, (cols + 3) / 4 * 4);
+      at[g] = a + min(s0 + g, slots - 1) * BM;
     }
-    store4(p, o, c, v, *reinterpret_cast<const float4*>(sx + c), cols - c);
+    for (int q = 0; q < parts; ++q)
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint4 w = at[g][q * slots * BM];
+        v[4 * g] += w.x; v[4 * g + 1] += w.y; v[4 * g + 2] += w.z; v[4 * g + 3] += w.w;
+      }
+    store_columns<G>(p, o, c, cols, v, sx);
   }
 }
 
@@ -179,8 +241,8 @@ struct Shape {
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = 108 * 1024 / STAGE;       // two CTAs per SM: the weight stream wants many loads in flight
   static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
-  static constexpr int SX = STAGES * STAGE + 256;         // [4 warps][BN] token scales (64 at least: fetched 32 at a time)
-  static constexpr int SMEM = SX + 4 * 64 * 4 + 1024;
+  static constexpr int SX = STAGES * STAGE + 256;         // [4 warps][NARROW_MAX + SX_PAD] token scales
+  static constexpr int SMEM = SX + 4 * (NARROW_MAX + SX_PAD) * 4 + 1024;
   static_assert(STAGES * 16 + 32 <= 256, "barrier area");
   static_assert((BN / 4 + MAX_SPLIT) * BM * 16 <= STAGES * STAGE, "partial sums over the ring");
 };
@@ -268,7 +330,7 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   const int r = quarter * 32 + lane;                       // channel row of this thread within the tile
   const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
   const int cols = min(BN, p.N - n0);                      // columns that hold a token
-  float* sx = reinterpret_cast<float*>(smem + S::SX) + quarter * 64;
+  float* sx = reinterpret_cast<float*>(smem + S::SX) + quarter * (NARROW_MAX + SX_PAD);
   bool have = false;
   if (warp >= 2) {
     fetch_sx(p, sx, n0, cols);
@@ -278,20 +340,13 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   }
   if (p.split == 1) {
     if (have) {
-      const OutWarp o(p, m0 + r, n0);
-      for (int c = 0; c < cols; c += 8) {
-        uint32_t v[8];
-        tmem_ld8(lane_base + c, v);
-        tmem_ld_wait();
-        store4(p, o, c, v, *reinterpret_cast<const float4*>(sx + c), cols - c);
-        if (c + 4 < cols) store4(p, o, c + 4, v + 4, *reinterpret_cast<const float4*>(sx + c + 4), cols - c - 4);
-      }
+      store_tile<4>(p, OutWarp(p, m0 + r, n0), lane_base, cols, sx, 0, 1);
     }
   } else {
     cluster_sync_all();                                    // every CTA's MMAs are done: the rings are free
-    if (warp >= 2) send_partials(smem_u32(smem), lane_base, have, cols, rank, p.split, r, [](int q) { return (uint32_t)q; });
+    if (warp >= 2) send_partials(smem_u32(smem), lane_base, have, cols, rank, p.split, r, 0, 1, [](int q) { return (uint32_t)q; });
     cluster_sync_all();
-    if (warp >= 2) finish_partials(p, smem, OutWarp(p, m0 + r, n0), sx, cols, rank, p.split, r);
+    if (warp >= 2) finish_partials<2>(p, smem, OutWarp(p, m0 + r, n0), sx, cols, rank, p.split, r, 0, 1);
   }
   if (*abort_flag && threadIdx.x == 0) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);       // let copies in flight land before the block ends
@@ -312,8 +367,10 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
 constexpr int PBN = 256;                                  // token tile at most; BN is any multiple of 32 up to it
 constexpr int P_RING = 192 * 1024;                        // stages of 16 KB + 64 * BN bytes
 constexpr int P_MAX_STAGES = 10;
-constexpr int P_SX = P_RING;                              // [4 warps][PBN] token scales
-constexpr int P_BARS = P_SX + 4 * PBN * 4;
+constexpr int P_EPI = 8;                                  // epilogue warps, two for each quarter of the channels
+constexpr int P_THREADS = 64 + 32 * P_EPI;
+constexpr int P_SX = P_RING;                              // [P_EPI warps][PBN + SX_PAD] token scales
+constexpr int P_BARS = P_SX + P_EPI * (PBN + SX_PAD) * 4;
 constexpr int P_SMEM = P_BARS + 256 + 1024;
 constexpr int PAIR_GROUP = 16;
 constexpr int PAIR_MAX_SPLIT = 4;
@@ -360,7 +417,7 @@ struct PairShape {
 };
 
 template <bool SPLIT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(P_THREADS, 1)
 gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constant__ CUtensorMap tm_w,
                       const __grid_constant__ CUtensorMap tm_x) {
   extern __shared__ uint8_t smem_raw[];
@@ -390,7 +447,7 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + i, 1);
-      mbar_init(acc_empty + i, 8);
+      mbar_init(acc_empty + i, 2 * P_EPI);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -410,7 +467,8 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
 
   const int quarter = warp & 3;
   const int r = quarter * 32 + lane;                                 // channel of this thread within the CTA's 128
-  float* sx = reinterpret_cast<float*>(smem + P_SX) + quarter * PBN;
+  const int turn = (warp - 2) >> 2;                                  // which of the quarter's two epilogue warps
+  float* sx = reinterpret_cast<float*>(smem + P_SX) + (warp - 2) * (PBN + SX_PAD);
   bool have = false;
   if (warp == 0) {
     if (elect_one()) {
@@ -490,14 +548,7 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
       tc_fence_after();
       if (SPLIT) break;
       const uint32_t acc = tmem + buf * PBN + ((uint32_t)(quarter * 32) << 16);
-      for (int c = 0; c < cols; c += 32) {
-        uint32_t v[32];
-        tmem_ld32(acc + c, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          if (c + i < cols) store4(p, o, c + i, v + i, *reinterpret_cast<const float4*>(sx + c + i), cols - c - i);
-      }
+      store_tile<4>(p, o, acc, cols, sx, turn, 2);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(acc_empty0 + buf * 8);
@@ -510,10 +561,10 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
     const int n0 = ni * sh.bn, cols = min(sh.bn, p.N - n0);
     cluster_sync_all();                                              // every CTA's MMAs are done: the rings are free
     if (warp >= 2)
-      send_partials(smem_u32(smem), tmem + ((uint32_t)(quarter * 32) << 16), have, cols, part, p.split, r,
+      send_partials(smem_u32(smem), tmem + ((uint32_t)(quarter * 32) << 16), have, cols, part, p.split, r, turn, 2,
                     [rank](int q) { return (uint32_t)(2 * q + rank); });
     cluster_sync_all();
-    if (warp >= 2) finish_partials(p, smem, OutWarp(p, mi * 2 * BM + rank * BM + r, n0), sx, cols, part, p.split, r);
+    if (warp >= 2) finish_partials<2>(p, smem, OutWarp(p, mi * 2 * BM + rank * BM + r, n0), sx, cols, part, p.split, r, turn, 2);
   }
   if (*abort_flag && threadIdx.x == 0) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);       // let copies in flight land before the block ends
@@ -587,7 +638,7 @@ const Room* room_of(int dev) {
     a.val.clusterDim.y = a.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(size * 256);
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(P_THREADS);
     cfg.dynamicSmemBytes = P_SMEM;
     cfg.attrs = &a;
     cfg.numAttrs = 1;
@@ -624,7 +675,7 @@ int launch_pair(const I8Params& p, const PairShape& sh, int sms, int dev, const 
   const int rc = allow_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<SPLIT>), P_SMEM, dev, done);
   if (rc) return rc;
   const int pairs = SPLIT ? sh.tiles.total * p.split : min(sms / 2, sh.tiles.total);
-  return (int)launch_pdl_cluster(gemm_int8_pair_kernel<SPLIT>, dim3(2 * pairs), dim3(THREADS), SPLIT ? 2u * p.split : 2u, P_SMEM, st, p,
+  return (int)launch_pdl_cluster(gemm_int8_pair_kernel<SPLIT>, dim3(2 * pairs), dim3(P_THREADS), SPLIT ? 2u * p.split : 2u, P_SMEM, st, p,
                                  sh, tw, tx);
 }
 
@@ -657,7 +708,7 @@ extern "C" int vg_gemm_int8(const void* codes, long long ldw, const float* sw, c
   CUtensorMap tw, tx;
   int rc = make_map(codes, M, K, ldw, BM, &tw);
   if (rc) return rc;
-  if (N <= 64) {
+  if (N <= NARROW_MAX) {
     const int bn = N <= 16 ? 16 : N <= 32 ? 32 : 64;
     const int tiles = (M + BM - 1) / BM;
     if (tiles > (1 << 26)) return -2;
