@@ -41,6 +41,11 @@ struct I8Params {
   int* err;
 };
 
+// A value that is the same in all lanes, in a form the compiler knows to be: branches on it and descriptors made from it
+// stay in uniform registers, which the MMA instructions need.
+template <typename T>
+VG_DEVINL T uniform(T v) { return (T)__shfl_sync(0xffffffffu, v, 0); }
+
 // Instruction descriptor: int32 accumulator, signed int8 operands, both K-major.
 constexpr uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -61,18 +66,6 @@ VG_DEVINL void dsmem_st_v4(uint32_t addr, const uint32_t* v) {
 VG_DEVINL void tma_prefetch_l2(const void* tmap, int c0, int c1) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tmap), "r"(c0), "r"(c1) : "memory");
 }
-VG_DEVINL void tmem_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-
 // Where a warp's stores go: 32 channels (this lane's is `m`) of the tokens from n0 on.
 struct OutWarp {
   char* base;               // vec: token (lane & 3), the first of the four channels around this lane; else token 0, channel m
@@ -259,14 +252,19 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = p.split > 1 ? (int)cluster_ctarank() : 0;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rank = p.split > 1 ? uniform((int)cluster_ctarank()) : 0;
   const int m0 = (blockIdx.x / p.split) * BM, n0 = blockIdx.y * BN;
   const int slabs = (p.K + BK - 1) / BK;
   const int s0 = (int)((long long)slabs * rank / p.split), s1 = (int)((long long)slabs * (rank + 1) / p.split);
   pdl_trigger();
 
-  if (threadIdx.x == 0) {
+  if (warp == 0 && elect_one()) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_x);
+    for (int s = s0; s < min(s1, s0 + S::STAGES); ++s) tma_prefetch_l2(&tm_w, s * BK, m0);
+  }
+  if (threadIdx.x == 64) {
     for (int i = 0; i < S::STAGES; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
@@ -274,8 +272,6 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tm_w);
-    tma_prefetch_desc(&tm_x);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, S::TMEM_COLS);
@@ -284,12 +280,11 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   auto fail = [&](int code) { if (p.err) atomicCAS(p.err, 0, code); *abort_flag = 1; };
 
   if (warp == 0) {
     if (elect_one()) {
-      for (int s = s0; s < min(s1, s0 + S::STAGES); ++s) tma_prefetch_l2(&tm_w, s * BK, m0);
       pdl_wait();
       int st = 0;
       uint32_t ph = 1;
@@ -365,8 +360,8 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
 // the group's tokens stay in L2.
 // Split K: a cluster of `split` pairs per tile, one tile per cluster.
 constexpr int PBN = 256;                                  // token tile at most; BN is any multiple of 32 up to it
-constexpr int P_RING = 192 * 1024;                        // stages of 16 KB + 64 * BN bytes
-constexpr int P_MAX_STAGES = 10;
+constexpr int P_RING = 216 * 1024;                        // stages of one or two slabs, 16 KB + 64 * BN bytes each
+constexpr int P_MAX_STAGES = 8;
 constexpr int P_EPI = 8;                                  // epilogue warps, two for each quarter of the channels
 constexpr int P_THREADS = 64 + 32 * P_EPI;
 constexpr int P_SX = P_RING;                              // [P_EPI warps][PBN + SX_PAD] token scales
@@ -412,7 +407,7 @@ struct PairTiles {
 };
 
 struct PairShape {
-  int bn, stage, stages;                                 // token tile, bytes of a ring stage, number of them
+  int bn, b_slab, per, stage, stages;                    // token tile, bytes of a CTA's token slab, slabs and bytes of a stage, stages
   PairTiles tiles;
 };
 
@@ -429,8 +424,8 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int crank = (int)cluster_ctarank();
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int crank = uniform((int)cluster_ctarank());
   const int rank = crank & 1, leader = crank & ~1;                   // within the pair / the pair's first CTA
   const int part = SPLIT ? crank >> 1 : 0;
   const int first = SPLIT ? (int)blockIdx.x / (2 * p.split) : (int)blockIdx.x >> 1;
@@ -440,7 +435,14 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   const int s1 = SPLIT ? (int)((long long)slabs * (part + 1) / p.split) : slabs;
   pdl_trigger();
 
-  if (threadIdx.x == 0) {
+  if (warp == 0 && elect_one()) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_x);
+    int mi, ni;
+    sh.tiles.at(first, mi, ni);
+    for (int s = s0; s < min(s1, s0 + sh.per * sh.stages); ++s) tma_prefetch_l2(&tm_w, s * BK, mi * 2 * BM + rank * BM);
+  }
+  if (threadIdx.x == 64) {
     for (int i = 0; i < sh.stages; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
@@ -451,8 +453,6 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
     }
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tm_w);
-    tma_prefetch_desc(&tm_x);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
@@ -462,7 +462,7 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   __syncthreads();
   cluster_sync_all();                                                // both CTAs' barriers are set up
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   auto fail = [&](int code) { if (p.err) atomicCAS(p.err, 0, code); *abort_flag = 1; };
 
   const int quarter = warp & 3;
@@ -473,10 +473,7 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   if (warp == 0) {
     if (elect_one()) {
       int mi, ni;
-      sh.tiles.at(first, mi, ni);
-      for (int s = s0; s < min(s1, s0 + sh.stages); ++s) tma_prefetch_l2(&tm_w, s * BK, mi * 2 * BM + rank * BM);
       pdl_wait();
-      const uint32_t tx = 2 * (uint32_t)sh.stage;
       const uint32_t full0 = dsmem_map(smem_u32(full), leader);
       int st = 0, issued = 0;
       uint32_t ph = 1;
@@ -484,12 +481,17 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
       for (int t = first; t < sh.tiles.total && ok; t += step) {
         sh.tiles.at(t, mi, ni);
         const int m0 = mi * 2 * BM + rank * BM, n0 = ni * sh.bn + rank * (sh.bn / 2);
-        for (int s = s0; s < s1; ++s) {
+        for (int s = s0; s < s1; s += sh.per) {
           if (!mbar_wait(empty + st, ph)) { fail(VG_ERR_EMPTY_WAIT); ok = false; break; }
-          const uint32_t a = smem_u32(smem) + st * sh.stage, bar = full0 + st * 8;
-          if (rank == 0) mbar_arrive_expect_tx(full + st, tx);
+          const uint32_t a = smem_u32(smem) + st * sh.stage, b = a + sh.per * A_BYTES, bar = full0 + st * 8;
+          const bool both = sh.per == 2 && s + 1 < s1;
+          if (rank == 0) mbar_arrive_expect_tx(full + st, (both ? 4 : 2) * (uint32_t)(A_BYTES + sh.b_slab));
           tma_pair_g2s(a, &tm_w, s * BK, m0, bar);
-          tma_pair_g2s(a + A_BYTES, &tm_x, s * BK, n0, bar);
+          tma_pair_g2s(b, &tm_x, s * BK, n0, bar);
+          if (both) {
+            tma_pair_g2s(a + A_BYTES, &tm_w, s * BK + BK, m0, bar);
+            tma_pair_g2s(b + sh.b_slab, &tm_x, s * BK + BK, n0, bar);
+          }
           ++issued;
           if (++st == sh.stages) { st = 0; ph ^= 1; }
         }
@@ -502,12 +504,14 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
       }
     }
   } else if (warp == 1) {
-    // The whole warp walks the loop and one elected lane issues: descriptors then stay in uniform registers. (With the
-    // loop inside a lane == 0 branch each MMA took 70 cycles to issue and a slab 330 more: 0.35 us a slab at any width.)
+    // The whole warp walks the loop and one elected lane issues. A stage costs 260 cycles of waiting, electing and
+    // committing whatever its size, and an MMA 10 more to issue: where a slab's MMAs take less, a stage holds two. (One
+    // slab a stage: 296 cycles a slab at any BN up to 128. With a warp index the compiler cannot know to be uniform, 388.
+    // With the loop inside a lane == 0 branch, 330 and 70 for each MMA.)
     if (rank == 0) {
       const uint32_t idesc = idesc_i8(2 * BM, sh.bn);
       const uint16_t mask = (uint16_t)(3u << leader);
-      const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), bdesc0 = umma_desc_sw128(smem_u32(smem) + A_BYTES);
+      const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), bdesc0 = umma_desc_sw128(smem_u32(smem) + sh.per * A_BYTES);
       int st = 0, it = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -516,16 +520,20 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
         if (!mbar_wait(acc_empty + buf, ((it >> 1) & 1) ^ 1)) { fail(VG_ERR_MMA_WAIT); break; }
         tc_fence_after();
         const uint32_t acc = tmem + buf * PBN;
-        for (int s = s0; s < s1; ++s) {
+        for (int s = s0; s < s1; s += sh.per) {
           if (!mbar_wait(full + st, ph)) { fail(VG_ERR_TMA_WAIT); ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t off = (uint64_t)(st * (sh.stage >> 4));
+            const uint64_t a = adesc0 + (uint64_t)(st * (sh.stage >> 4)), b = bdesc0 + (uint64_t)(st * (sh.stage >> 4));
 #pragma unroll
-            for (int kk = 0; kk < BK / 32; ++kk)
-              umma_i8_pair(acc, adesc0 + off + kk * 2, bdesc0 + off + kk * 2, idesc, (s > s0 || kk) ? 1u : 0u);
+            for (int kk = 0; kk < BK / 32; ++kk) umma_i8_pair(acc, a + kk * 2, b + kk * 2, idesc, (s > s0 || kk) ? 1u : 0u);
+            if (sh.per == 2 && s + 1 < s1) {
+              const uint64_t a1 = a + (A_BYTES >> 4), b1 = b + (uint64_t)(sh.b_slab >> 4);
+#pragma unroll
+              for (int kk = 0; kk < BK / 32; ++kk) umma_i8_pair(acc, a1 + kk * 2, b1 + kk * 2, idesc, 1u);
+            }
             umma_commit_pair(empty + st, mask);
-            if (s == s1 - 1) umma_commit_pair(acc_full + buf, mask);
+            if (s + sh.per >= s1) umma_commit_pair(acc_full + buf, mask);
           }
           __syncwarp();
           if (++st == sh.stages) { st = 0; ph ^= 1; }
@@ -648,17 +656,24 @@ const Room* room_of(int dev) {
   return &room;
 }
 
-// Token tile and K split of the pair form: the shape with the least estimated time, in cycles.
-void choose_pair(int N, int slabs, const Room& room, PairShape* sh, int* split) {
-  const int least = (N + PBN - 1) / PBN;
+// Token tile and K split of the pair form: the shape with the least estimated time (us), from tiles of 64 tokens up.
+// Fitted to single rounds of 20 - 60 tiles at K = 6144 and 17408: a slab takes 0.157 us at 64 tokens (waiting and copying),
+// 0.19 at 128, 0.30 at 256 (MMAs: 512 cycles and the epilogue's share); a launch 3.6 us and 6 ns a token of its tiles,
+// 5 us more when partial sums travel. Splitting pays where there are few tiles and much K: 256 x 5120 x 17408 46.0 us
+// whole with 256-token tiles, 28.6 with 96, 26.7 split three ways; at K = 6144 12.9 with 96, 16.3 split.
+void choose_pair(int N, int K, int M, const Room& room, PairShape* sh, int* split) {
+  const int slabs = (K + BK - 1) / BK, least = (N + PBN - 1) / PBN;
+  const double weights = (double)M * K / 6.2e6;                 // from memory at 6.2 TB/s
   double best = 1e30;
-  for (int nt = least; nt < least + 4; ++nt) {
-    const int bn = ((N + nt - 1) / nt + 31) / 32 * 32;
+  sh->tiles.mt = (M + 2 * BM - 1) / (2 * BM);
+  for (int nt = least; nt <= min(4 * least, least + 6); ++nt) {
+    const int bn = max(64, ((N + nt - 1) / nt + 31) / 32 * 32);
     const int used = (N + bn - 1) / bn;
-    const double slab = max(2.0 * bn, 195 + 0.76 * bn);
+    const double slab = max(0.125 + 0.0005 * bn, 0.00117 * bn);
     for (int s = 1; s <= PAIR_MAX_SPLIT && s <= max(1, slabs / 4); ++s) {
-      const double waves = ceil((double)sh->tiles.mt * used / max(1, room.clusters[2 * s]));
-      const double t = waves * ((slabs + s - 1) / s) * slab + (s > 1 ? waves * (4000 + 12.0 * bn) : 2000 + 12.0 * bn);
+      const double rounds = ceil((double)sh->tiles.mt * used / max(1, room.clusters[2 * s]));
+      const double work = rounds * ((slabs + s - 1) / s) * slab, fixed = 3.6 + 0.006 * bn;
+      const double t = max(work, weights) + (s > 1 ? rounds * (fixed + 4.0 + 0.5 * s) : fixed);
       if (t < best) {
         best = t;
         sh->bn = bn;
@@ -667,6 +682,10 @@ void choose_pair(int N, int slabs, const Room& room, PairShape* sh, int* split) 
       }
     }
   }
+  sh->b_slab = sh->bn / 2 * BK;
+  sh->per = sh->bn < 160 ? 2 : 1;
+  sh->stage = sh->per * (A_BYTES + sh->b_slab);
+  sh->stages = min(P_MAX_STAGES, P_RING / sh->stage);
 }
 
 template <bool SPLIT>
@@ -725,10 +744,7 @@ extern "C" int vg_gemm_int8(const void* codes, long long ldw, const float* sw, c
     }
   }
   PairShape sh{};
-  sh.tiles.mt = (M + 2 * BM - 1) / (2 * BM);
-  choose_pair(N, slabs, *room, &sh, &p.split);
-  sh.stage = A_BYTES + sh.bn / 2 * BK;
-  sh.stages = min(P_MAX_STAGES, P_RING / sh.stage);
+  choose_pair(N, K, M, *room, &sh, &p.split);
   if ((long long)sh.tiles.mt * sh.tiles.nt > (1 << 26)) return -2;
   sh.tiles.total = sh.tiles.mt * sh.tiles.nt;
   rc = make_map(q, N, K, ldq, sh.bn / 2, &tx);
