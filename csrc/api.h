@@ -104,7 +104,7 @@ int vg_add_rmsnorm_int8(void* res, long long ld_res, const void* delta, long lon
                         float eps, int plus_one, void* q, long long ldq, float* scale, void* out16, long long ld_out16,
                         int* err, cudaStream_t stream);
 int vg_dequant_int8(const void* q, long long ldq, const float* scale, void* out, long long ldo, int dtype, int n, int k,
-                    cudaStream_t stream);
+                    int* err, cudaStream_t stream);
 int vg_gemm_int8(const void* codes, long long ldw, const float* sw, const void* q, long long ldq, const float* sx, void* out,
                  long long ldo, int out_f32, int M, int K, int N, int* err, cudaStream_t stream);
 

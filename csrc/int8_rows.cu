@@ -649,7 +649,7 @@ extern "C" int vg_add_rmsnorm_int8(void* res, long long ld_res, const void* delt
 }
 
 extern "C" int vg_dequant_int8(const void* q, long long ldq, const float* scale, void* out, long long ldo, int dtype, int n,
-                               int k, cudaStream_t st) {
+                               int k, int*, cudaStream_t st) {
   if (k <= 0 || n < 0) return -2;
   if (n == 0) return 0;
   const signed char* c = static_cast<const signed char*>(q);

@@ -41,74 +41,80 @@ def act_buffers(rows: int, k: int, device) -> Int8Act:
     return Int8Act(q if kp == k else q[:, :k], torch.empty(rows, dtype=torch.float32, device=device))
 
 
+# argument types of the C entries, set once so that plain ints and floats convert without wrapper objects
+_P, _I, _L, _F = c_void_p, c_int, c_ll, c_float
+_TYPES = {"vg_quant_int8": (_P, _L, _I, _I, _I, _P, _L, _P, _P, _P),
+          "vg_swiglu_int8": (_P, _L, _I, _I, _P, _L, _P, _P, _P),
+          "vg_add_rmsnorm_int8": (_P, _L, _P, _L, _P, _I, _I, _F, _I, _P, _L, _P, _P, _L, _P, _P),
+          "vg_dequant_int8": (_P, _L, _P, _P, _L, _I, _I, _I, _P, _P),
+          "vg_gemm_int8": (_P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _P, _P)}
 _fns = {}
+_devices = {}                  # CUDA device -> (index, address of its error word)
 
 
 def _fn(name: str):
-    """C entry with its argument types set once (plain ints and floats then convert without wrapper objects)."""
-    f = _fns.get(name)
-    if f is None:
-        P, I, L, F = c_void_p, c_int, c_ll, c_float
-        types = {"vg_quant_int8": (P, L, I, I, I, P, L, P, P, P),
-                 "vg_swiglu_int8": (P, L, I, I, P, L, P, P, P),
-                 "vg_add_rmsnorm_int8": (P, L, P, L, P, I, I, F, I, P, L, P, P, L, P, P),
-                 "vg_dequant_int8": (P, L, P, P, L, I, I, I, P),
-                 "vg_gemm_int8": (P, L, P, P, L, P, P, L, I, I, I, I, P, P)}[name]
-        f = getattr(_lib.lib(), name)
-        f.argtypes = types
-        f.restype = c_int
-        _fns[name] = f
+    f = getattr(_lib.lib(), name)
+    f.argtypes = _TYPES[name]
+    f.restype = c_int
+    _fns[name] = f
     return f
 
 
+def _device(device: torch.device):
+    if device.type != "cuda":
+        raise KernelError(f"the 8-bit integer path runs on CUDA tensors, got {device}")
+    d = _devices[device] = (device.index, _lib.err_word(device).data_ptr())
+    return d
+
+
 def _launch(name: str, device: torch.device, *args):
-    index = device.index
-    if index is None or device.type != "cuda":
-        raise KernelError(f"{name[3:]} runs on CUDA tensors, got {device}")
-    if index == torch.cuda.current_device():
-        _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name)
+    """Enqueues on the current stream of ``device``; every entry ends with (error word, stream)."""
+    index, err = _devices.get(device) or _device(device)
+    fn = _fns.get(name) or _fn(name)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            _lib.check(fn(*args, err, _lib.raw_stream(index)), name)
         return
-    with torch.cuda.device(index):
-        _lib.check(_fn(name)(*args, _lib.raw_stream(index)), name)
-
-
-_err_ptrs = {}
-
-
-def _err(device: torch.device) -> int:
-    p = _err_ptrs.get(device)
-    if p is None:
-        if device.type != "cuda":
-            return 0                                    # refused by _launch
-        p = _err_ptrs[device] = _lib.err_word(device).data_ptr()
-    return p
+    _lib.check(fn(*args, err, _lib.raw_stream(index)), name)
 
 
 def _input(t: torch.Tensor, what: str, dtypes, n: Optional[int]):
     """Rows to process, row width and row pitch of a call's main argument."""
-    if t.dim() != 2:
-        raise KernelError(f"{what}: expected a matrix, got shape {tuple(t.shape)}")
-    rows, cols = t.shape
+    shape = t.shape
+    if len(shape) != 2:
+        raise KernelError(f"{what}: expected a matrix, got shape {tuple(shape)}")
+    rows, cols = shape
     if n is None:
         n = rows
     if not 0 <= n <= rows or n > MAX_ROWS:
         raise KernelError(f"{what}: {n} rows asked for, the tensor has {rows}")
-    return n, cols, _matrix(t, what, dtypes, n, cols)
+    if t.dtype not in dtypes:
+        raise KernelError(f"{what}: dtype {t.dtype} is not supported")
+    ld, inner = t.stride()
+    if inner != 1 or ld < cols:
+        ld = _pitch(t, what, n, cols)
+    return n, cols, ld
 
 
-def _matrix(t: torch.Tensor, what: str, dtypes, rows: int, cols: int, device=None) -> int:
+def _pitch(t: torch.Tensor, what: str, rows: int, cols: int) -> int:
+    """Row pitch of a matrix whose strides are not plainly row-major: single rows and columns may have any."""
+    ld, inner = t.stride()
+    if (inner != 1 and cols > 1) or (ld < cols and rows > 1):
+        raise KernelError(f"{what}: rows must be contiguous and must not overlap (strides {t.stride()})")
+    return ld if rows > 1 else max(ld, cols)
+
+
+def _matrix(t: torch.Tensor, what: str, dtypes, rows: int, cols: int, device) -> int:
     """Row pitch of a 2-D row-major argument that has to hold ``rows`` x ``cols`` elements."""
     if t.dtype not in dtypes:
         raise KernelError(f"{what}: dtype {t.dtype} is not supported")
     shape = t.shape
     if len(shape) != 2 or shape[0] < rows or shape[1] != cols:
         raise KernelError(f"{what}: shape {tuple(shape)}, expected at least {rows} rows of {cols}")
-    if device is not None and t.device != device:
+    if t.device != device:
         raise KernelError(f"{what} is on {t.device}, expected {device}")
     ld, inner = t.stride()
-    if (inner != 1 and cols > 1) or (ld < cols and rows > 1):
-        raise KernelError(f"{what}: rows must be contiguous and must not overlap (strides {t.stride()})")
-    return ld if rows > 1 else max(ld, cols)
+    return ld if inner == 1 and ld >= cols else _pitch(t, what, rows, cols)
 
 
 def _vector(t: torch.Tensor, what: str, size: int, device, least: bool = False):
@@ -134,7 +140,7 @@ def quantize_act_int8(x: torch.Tensor, n: Optional[int] = None, out: Optional[In
     dev = x.device
     out, ldq = _out(out, n, k, dev)
     if n:
-        _launch("vg_quant_int8", dev, x.data_ptr(), ld, _DTYPE[x.dtype], n, k, out.q.data_ptr(), ldq, out.scale.data_ptr(), _err(dev))
+        _launch("vg_quant_int8", dev, x.data_ptr(), ld, _DTYPE[x.dtype], n, k, out.q.data_ptr(), ldq, out.scale.data_ptr())
     return out
 
 
@@ -148,7 +154,7 @@ def swiglu_int8(gu: torch.Tensor, n: Optional[int] = None, inter: Optional[int] 
     dev = gu.device
     out, ldq = _out(out, n, inter, dev)
     if n:
-        _launch("vg_swiglu_int8", dev, gu.data_ptr(), ld, n, inter, out.q.data_ptr(), ldq, out.scale.data_ptr(), _err(dev))
+        _launch("vg_swiglu_int8", dev, gu.data_ptr(), ld, n, inter, out.q.data_ptr(), ldq, out.scale.data_ptr())
     return out
 
 
@@ -170,7 +176,7 @@ def add_rmsnorm_int8(res: torch.Tensor, delta: Optional[torch.Tensor], w: torch.
     if n:
         _launch("vg_add_rmsnorm_int8", dev, res.data_ptr(), ld, 0 if delta is None else delta.data_ptr(), ldd, w.data_ptr(), n, h,
                 eps, 1 if plus_one else 0, out.q.data_ptr(), ldq, out.scale.data_ptr(),
-                0 if out16 is None else out16.data_ptr(), ldo, _err(dev))
+                0 if out16 is None else out16.data_ptr(), ldo)
     return out
 
 
@@ -223,5 +229,5 @@ def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional
         ldo = _matrix(out, "out", (torch.bfloat16, torch.float32), n, m, dev)
     if n:
         _launch("vg_gemm_int8", dev, wp, ldw, q.row_scale.data_ptr(), qp, ldq, act.scale.data_ptr(), out.data_ptr(), ldo,
-                1 if out.dtype == torch.float32 else 0, m, k, n, _err(dev))
+                1 if out.dtype == torch.float32 else 0, m, k, n)
     return out
