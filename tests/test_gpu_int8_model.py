@@ -1,0 +1,109 @@
+"""Models whose dense linears run on the 8-bit integer path (weights and activations), against the fp32 oracle, and the
+engine's bitwise properties on it."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+RECIPE = "all,mlp:int8,attn:int8,gdn:int8"
+
+
+def _build(moe=False, recipe=RECIPE):
+    from velogb10_b200.checkpoint.synthetic import SyntheticSource
+    from velogb10_b200.config import tiny_hybrid, tiny_moe
+    from velogb10_b200.models.weights import ModelBuilder
+    cfg = tiny_moe() if moe else tiny_hybrid()
+    return cfg, ModelBuilder(cfg, SyntheticSource(cfg, 0, "cuda", std=0.05), recipe=recipe, device="cuda").build()
+
+
+def _prompt(cfg, n, seed=1):
+    return torch.randint(0, cfg.vocab_size, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+# Rounding an input to 8 bits adds noise of step / sqrt(12) with step = max / 127: 0.75 % of a 256-wide Gaussian row, about
+# 2 % of a SwiGLU row (largest value 8 times the rms). The branches' errors add like the branches themselves, so logits made
+# from the same weight codes and unquantised activations differ by about 2 %: 6 % is three times that.
+NOISE = 0.06
+
+
+def test_prefill_and_decode_match_oracle():
+    from velogb10_b200.models.oracle import OracleModel
+    from velogb10_b200.models.runtime import GpuModel
+    from velogb10_b200.ops import lib
+    cfg, w = _build()
+    orc = OracleModel(_build()[1])
+    gm = GpuModel(w, keep_canonical=True)
+    assert {q.fmt for _, q in w.linears()} >= {"int8", "nvfp4"}
+    gm.alloc_state(2, 2 + 17, 256)
+    orc.alloc_state(2, 2 + 17, 256)
+    prompt = _prompt(cfg, 40)
+    lg, _ = gm.prefill(1, prompt)
+    lo, _ = orc.prefill(1, prompt)
+    assert ((lg.float().cpu() - lo).norm() / lo.norm()).item() < NOISE
+    tok = int(lo.argmax())
+    for i in range(3):
+        lgd, _ = gm.decode([tok], [40 + i], [1])
+        lod, _ = orc.decode([tok], [40 + i], [1])
+        assert ((lgd[0].float().cpu() - lod[0]).norm() / lod[0].norm()).item() < NOISE
+        tok = int(lod[0].argmax())
+    lib.check_err_word()
+
+
+def test_moe_with_int8_mixers_and_shared_expert():
+    """Expert selection is a step function of the router logits, so noise in them changes outputs without bound: the
+    reference (the same codes decoded to bf16) lends its router logits to the int8 run."""
+    from velogb10_b200.models.runtime import GpuModel
+    from velogb10_b200.ops import lib
+    cfg, w = _build(moe=True)
+    ref = _build(moe=True)[1]
+    for _, q in ref.linears():
+        if q.fmt == "int8":
+            q.w, q.fmt, q.codes, q.row_scale = q.dequant(torch.bfloat16), "bf16", None, None
+    a, b = GpuModel(w, keep_canonical=True), GpuModel(ref, keep_canonical=True)
+    for m in (a, b):
+        m.alloc_state(2, 2 + 17, 256)
+    seen = []
+    b.router_logits_hook = lambda logits, n: seen.append(logits[:n].clone())
+    a.router_logits_hook = lambda logits, n: logits[:n].copy_(seen.pop(0))
+    prompt = _prompt(cfg, 40)
+    want = b.prefill(1, prompt)[0].clone()
+    got = a.prefill(1, prompt)[0]
+    assert ((got.float() - want.float()).norm() / want.float().norm()).item() < NOISE
+    for i, tok in enumerate((3, 77, 500)):
+        want = b.decode([tok], [40 + i], [1])[0].clone()
+        got = a.decode([tok], [40 + i], [1])[0]
+        assert ((got.float() - want.float()).norm() / want.float().norm()).item() < NOISE
+    assert not seen
+    lib.check_err_word()
+
+
+def test_batch_verify_and_graph_are_bitwise_sequential():
+    from velogb10_b200.models.runtime import GpuModel
+    cfg, w = _build()
+    gm = GpuModel(w, keep_canonical=True)
+    gm.alloc_state(4, 4 + 17, 512)
+    prompts = [_prompt(cfg, n, n) for n in (16, 23, 70, 33)]
+    firsts = [int(gm.prefill(s, p)[0].argmax()) for s, p in enumerate(prompts)]
+    keep = [t.clone() for t in (gm.S, gm.conv, gm.kc, gm.vc)]
+
+    def restore():
+        for t, k in zip((gm.S, gm.conv, gm.kc, gm.vc), keep):
+            t.copy_(k)
+
+    pos = [len(p) for p in prompts]
+    batch = gm.decode(firsts, pos, [0, 1, 2, 3])[0].clone()
+    restore()
+    for s in range(4):
+        assert torch.equal(gm.decode([firsts[s]], [pos[s]], [s])[0][0], batch[s]), s
+    restore()
+    toks = [firsts[2], 5, 7, 11]
+    verify = gm.verify(2, toks, pos[2], ckpt_base=4)[0].clone()
+    restore()
+    for t in range(4):
+        assert torch.equal(gm.decode([toks[t]], [pos[2] + t], [2])[0][0], verify[t]), t
+    restore()
+    gm.capture_decode(4)
+    restore()
+    gm.replay_decode(firsts, pos, [0, 1, 2, 3])
+    torch.cuda.synchronize()
+    assert gm.ws.out_tok[:4].tolist() == batch.argmax(-1).tolist()

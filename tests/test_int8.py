@@ -49,6 +49,43 @@ def test_container_keeps_rows_on_16_byte_boundaries():
     assert mixed.fmt == "bf16"
 
 
+def test_recipe_and_checkpoint(tmp_path):
+    from velogb10_b200.checkpoint import io
+    from velogb10_b200.checkpoint.synthetic import SyntheticSource, synthetic_state_dict
+    from velogb10_b200.config import tiny_hybrid
+    from velogb10_b200.models.weights import ModelBuilder
+    from velogb10_b200.quant.recipe import parse_recipe
+    recipe = "all,mlp:int8,attn:int8,gdn:int8"
+    assert parse_recipe(recipe)["mlp"] == "int8" and parse_recipe(recipe)["lmhead"] == "nvfp4"
+    assert "mlp" not in parse_recipe("mlp:int8,-mlp:int8")
+    for bad in ("all:int8", "lmhead:int8", "expert:int8", "embed:int8", "router:int8", "mtp:int8"):
+        with pytest.raises(ValueError, match="int8 is for"):
+            parse_recipe(bad)
+    cfg = tiny_hybrid(False)
+    out = str(tmp_path / "ck")
+    stats = io.write_checkpoint(out, synthetic_state_dict(cfg, seed=0).items(), cfg.to_hf_dict(), recipe)
+    assert stats["int8"] > 0 and stats["nvfp4"] > 0
+    direct = ModelBuilder(cfg, SyntheticSource(cfg, 0), recipe=recipe).build()
+    loaded = ModelBuilder(cfg, io.SafetensorsSource(out)).build()
+    n = 0
+    for (name, a), (name2, b) in zip(direct.linears(), loaded.linears()):
+        assert name == name2 and a.fmt == b.fmt
+        if a.fmt == "int8":
+            n += 1
+            assert torch.equal(a.codes, b.codes) and torch.equal(a.row_scale, b.row_scale)
+            assert b.codes.stride(0) % 16 == 0 and b.codes.data_ptr() % 16 == 0
+    assert n == 2 * cfg.num_layers + 2 * cfg.num_layers          # mixer in / out and MLP in / down of every layer
+
+
+def test_other_linears_refuse_int8_weights():
+    from velogb10_b200.ops import gemm as G
+    q = _w(16, 32)
+    with pytest.raises(KernelError, match="int8"):
+        G.prepare(q)
+    with pytest.raises(KernelError, match="int8"):
+        G.linear_simt(q, torch.zeros(1, 32, dtype=torch.float16))
+
+
 def _act(n, k):
     return I8.Int8Act(codec.rows16(torch.zeros((n, k), dtype=torch.int8)), torch.ones(n))
 

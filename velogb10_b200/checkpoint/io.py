@@ -321,6 +321,11 @@ def emit_tensor(w: ShardWriter, name: str, t: torch.Tensor, recipe: Optional[dic
         w.add(stem + ".weight_scale", q.scales.view(torch.float8_e4m3fn))
         w.add(stem + ".weight_global_scale", torch.tensor([q.global_scale], dtype=torch.float32))
         stats["nvfp4"] += 1
+    elif fmt == "int8":
+        qi = codec.quantize_int8(w2)
+        w.add(stem + ".weight", qi.codes.contiguous())
+        w.add(stem + ".weight_scale", qi.row_scale)
+        stats["int8"] = stats.get("int8", 0) + 1
     else:
         q8 = codec.quantize_fp8(w2)
         w.add(stem + ".weight", q8.codes.view(torch.float8_e4m3fn))

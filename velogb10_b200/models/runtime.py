@@ -19,6 +19,7 @@ import torch
 
 from ..config import ModelConfig
 from ..ops import gemm as G
+from ..ops import int8 as I8
 from ..ops import kernels as K
 from ..ops import lib as _lib
 from .weights import LayerW, ModelWeights, MoeW, QLinear
@@ -126,6 +127,7 @@ class Workspace:
             if L.moe and L.moe.shared:
                 widths.append(L.moe.shared.gate_up.m)
         self.wide = bf(rows, (max(widths) + 63) // 64 * 64)                 # qkv / in_proj / gate_up outputs
+        self._i8 = {}                                     # int8 GEMM-input buffers by (width, tag)
         self._a16 = {}                                    # contiguous f16 GEMM-input buffers by width
         self._rows, self._dev = rows, dev
         nh_max = max([L.attn.nh for L in list(w.layers) + ([w.mtp.layer] if w.mtp else []) if L.attn] or [1])
@@ -141,6 +143,13 @@ class Workspace:
             self.mtp_e = bf(rows, h)
         self.n_uploaded = 0
         self.upload_done = None
+
+    def i8(self, width: int, tag: str = ""):
+        """Quantised-token buffers (codes and scales) of an int8 linear's input; a second stream uses its own ``tag``."""
+        t = self._i8.get((width, tag))
+        if t is None:
+            t = self._i8[(width, tag)] = I8.act_buffers(self._rows, width, self._dev)
+        return t
 
     def a16(self, width: int) -> torch.Tensor:
         """Contiguous f16 ``[rows, width]`` buffer that receives attention / GDN / SwiGLU outputs."""
@@ -222,7 +231,7 @@ class GpuModel:
                 if small and q.experts <= 1 and q.w is not None and name.endswith(("router", "shared_gate")):
                     G.prepare(q, keep_canonical=True)        # f16 tiles for prefill widths; decode keeps the GEMV
                     continue
-                if small or q.experts > 1:
+                if small or q.experts > 1 or q.fmt == "int8":        # int8 weights are read as they are
                     continue
                 if self.use_fp4 and q.fmt == "nvfp4" and q.packed is not None:
                     G.prepare_fp4(q)
@@ -387,31 +396,49 @@ class GpuModel:
     def _fp4_ok(self, q: QLinear, n: int) -> bool:
         return self.use_fp4 and n <= 16 and getattr(q, "kernel4", None) is not None
 
-    def _norm(self, ws: Workspace, delta, w: torch.Tensor, n: int):
+    def _norm(self, ws: Workspace, delta, w: torch.Tensor, n: int, q: Optional[QLinear] = None):
         """Residual add + RMSNorm into ``ws.xn16``; at decode widths the same kernel also emits the FP4
         activation series, returned for the linears that read this input. When the preceding row-parallel
         linear only pushed its partial rows (``self._pending_ar``), the kernel also performs the
-        tensor-parallel sum."""
+        tensor-parallel sum. When the linear ``q`` that reads the result has int8 weights, the same kernel emits
+        int8 rows instead."""
         if self._pending_ar:
             mode, self._pending_ar = self._pending_ar, 0
             return G.add_rmsnorm_fp4_ar(ws.x, w, self.cfg.rms_eps, n, self.comm, out16=ws.xn16, mode=mode)
+        if q is not None and q.fmt == "int8":
+            return I8.add_rmsnorm_int8(ws.x, delta, w, self.cfg.rms_eps, n, out=ws.i8(ws.x.shape[1]), out16=ws.xn16)
         if self.use_fp4 and n <= 16 and ws.x.shape[1] % 16 == 0:
             return G.add_rmsnorm_fp4(ws.x, delta, w, self.cfg.rms_eps, n, out16=ws.xn16)
         K.add_rmsnorm(ws.x, delta, w, self.cfg.rms_eps, n, out16=ws.xn16)
         return None
 
     def _linear(self, q: QLinear, x16: torch.Tensor, n: int, out: torch.Tensor, act=None, out_f32: bool = False,
-                comm=None):
-        if self._fp4_ok(q, n):
+                comm=None, ws: Optional[Workspace] = None, tag: str = ""):
+        """``act``: the input already quantised for this linear's path (FP4 series or int8 rows), else it is made here
+        (int8: into buffers of ``ws``, or of the call)."""
+        if q.fmt == "int8":
+            assert comm is None
+            if not isinstance(act, I8.Int8Act):
+                act = I8.quantize_act_int8(x16, n, out=ws.i8(q.k, tag) if ws is not None else None)
+            I8.linear_int8(q, act, n, out=out)
+        elif self._fp4_ok(q, n):
+            if isinstance(act, I8.Int8Act):
+                act = None
             G.linear_fp4(q, x16, n, out=out, out_f32=out_f32, comm=comm, act=act)
         else:
             G.linear(q, x16, n, out=out, out_f32=out_f32, comm=comm)
 
-    def _row_parallel(self, q: QLinear, x16: torch.Tensor, n: int, out: torch.Tensor, reduce: bool = True, act=None):
+    def _row_parallel(self, q: QLinear, x16: torch.Tensor, n: int, out: torch.Tensor, reduce: bool = True, act=None,
+                      ws: Optional[Workspace] = None, tag: str = ""):
         """Row-parallel linear + tensor-parallel sum. For decode / verify widths the reduction is fused into
         the GEMM epilogue (peer-memory pushes + flags inside the same kernel); longer inputs run the GEMM and
         then the two-shot peer-memory all-reduce."""
         tp = reduce and self.comm is not None and self.comm.world > 1
+        if q.fmt == "int8":
+            self._linear(q, x16, n, out, act=act, ws=ws, tag=tag)
+            if tp:
+                self._reduce(out, n)
+            return
         if tp and n <= 16 and not self.comm.use_nccl and self.fuse_allreduce and (q.m + 127) // 128 <= 64:
             # (a reduced row-parallel output is always the delta the next residual-add / RMSNorm consumes)
             if self.split_allreduce and self._fp4_ok(q, n) and q.m == self.cfg.hidden_size and q.m % 16 == 0:
@@ -451,7 +478,7 @@ class GpuModel:
     def _attn(self, ws: Workspace, L: LayerW, n: int, kc, vc, plan_direct: bool, use_path: bool, act=None):
         c, A = self.cfg, L.attn
         qkv = ws.wide[:, :A.qkv.m]
-        self._linear(A.qkv, ws.xn16, n, qkv, act=act)
+        self._linear(A.qkv, ws.xn16, n, qkv, act=act, ws=ws)
         ksc, vsc = self._kv_scales if self._kv_scales is not None else (None, None)
         K.attn_prep(qkv, A.q_norm, A.k_norm, ws.pos, ws.kv_slot, ws.kv_row, ws.q, kc, vc, n, A.nh, A.nkv,
                     c.head_dim, c.rotary_dim, c.rms_eps, c.rope_theta, c.attn_out_gate, k_scale=ksc, v_scale=vsc)
@@ -477,7 +504,7 @@ class GpuModel:
                           gate=qkv if c.attn_out_gate else None, base=ws.base if use_path else None,
                           path=ws.path if use_path else None, ns_grid=self.ns_grid, direct=plan_direct,
                           k_scale=ksc, v_scale=vsc)
-        self._row_parallel(A.o, a16, n, ws.delta)
+        self._row_parallel(A.o, a16, n, ws.delta, ws=ws)
 
     def _gdn(self, ws: Workspace, L: LayerW, li: int, n: int, n_chains: int, seq_mode: bool, act=None):
         c, Gd = self.cfg, L.gdn
@@ -492,7 +519,7 @@ class GpuModel:
                                 c.conv_kernel)
             G.linear_fp4(Gd.in_proj, ws.xn16, n, out=proj, act=act, conv=cv)
         elif seq_mode:
-            self._linear(Gd.in_proj, ws.xn16, n, proj, act=act)
+            self._linear(Gd.in_proj, ws.xn16, n, proj, act=act, ws=ws)
             if not (linear_chain and K.gdn_conv_chain(proj, self.conv[gi], Gd.conv_w, ws.st_in, ws.parent, ws.st_out,
                                                       ws.conv_out, n, conv_dim, c.conv_kernel)):
                 K.gdn_conv(proj, self.conv[gi], Gd.conv_w, ws.st_in, ws.parent, ws.st_out, ws.conv_out, n, conv_dim,
@@ -500,7 +527,7 @@ class GpuModel:
                 K.gdn_conv(proj, self.conv[gi], Gd.conv_w, ws.st_in, ws.parent, ws.st_out, ws.conv_out, n, conv_dim,
                            c.conv_kernel, phase=2)
         else:
-            self._linear(Gd.in_proj, ws.xn16, n, proj, act=act)
+            self._linear(Gd.in_proj, ws.xn16, n, proj, act=act, ws=ws)
             K.gdn_conv(proj, self.conv[gi], Gd.conv_w, ws.st_in, ws.parent, ws.st_out, ws.conv_out, n, conv_dim,
                        c.conv_kernel, phase=3)
         g16 = ws.a16(Gd.out.k)
@@ -538,14 +565,18 @@ class GpuModel:
                        Gd.A_log, Gd.dt_bias, Gd.norm, ws.chain_start, ws.chain_len, n_chains, ws.st_in, ws.parent,
                        ws.st_out, g16, Gd.nk, Gd.nv, c.lin_k_dim, c.lin_v_dim, c.rms_eps,
                        quant=act_o + (self.col_ctr,) if act_o is not None else None)
-        self._row_parallel(Gd.out, g16, n, ws.delta, act=act_o)
+        self._row_parallel(Gd.out, g16, n, ws.delta, act=act_o, ws=ws)
 
     def _mlp(self, ws: Workspace, M, n: int, out: torch.Tensor, reduce: bool = True, act=None, buf_tag: str = ""):
         """SwiGLU MLP. ``buf_tag`` selects a private set of FP4 activation buffers (an MLP that runs on a second
         stream must not share them with the main stream's producers)."""
         gu = ws.wide[:, :M.gate_up.m]
-        self._linear(M.gate_up, ws.xn16, n, gu, act=act)
+        self._linear(M.gate_up, ws.xn16, n, gu, act=act, ws=ws, tag=buf_tag)
         a16 = ws.a16(M.down.k)
+        if M.down.fmt == "int8":
+            act_d = I8.swiglu_int8(gu, n, M.inter, out=ws.i8(M.inter, buf_tag))
+            self._row_parallel(M.down, a16, n, out, reduce, act=act_d)
+            return
         if self._fp4_ok(M.down, n) and M.inter % 8 == 0:
             bufs = G.fp4_buffers(self.dev, ((M.inter + 255) // 256) * 256, tag=buf_tag) if buf_tag else None
             act_d = G.swiglu_fp4(gu, n, M.inter, bufs=bufs)
@@ -560,7 +591,7 @@ class GpuModel:
 
     def _layer(self, ws, L: LayerW, li, n, n_chains, seq_mode, direct, use_path, kc, vc, first_delta):
         c = self.cfg
-        act = self._norm(ws, first_delta, L.input_norm, n)
+        act = self._norm(ws, first_delta, L.input_norm, n, L.attn.qkv if L.attn is not None else L.gdn.in_proj)
         if self.cap_debug:
             self._cap_debug(f"layer {li} normed", ws.xn16, n)
         if L.attn is not None:
@@ -569,7 +600,7 @@ class GpuModel:
             self._gdn(ws, L, li, n, n_chains, seq_mode, act=act)
         if self.cap_debug and not self._pending_ar:
             self._cap_debug(f"layer {li} mixer out", ws.delta, n)
-        act = self._norm(ws, ws.delta, L.post_norm, n)
+        act = self._norm(ws, ws.delta, L.post_norm, n, L.mlp.gate_up if L.moe is None else None)
         if L.moe is not None:
             self._moe(ws, L.moe, n, act=act)
         else:

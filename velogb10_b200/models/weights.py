@@ -358,6 +358,10 @@ class ModelBuilder:
             c = w.view(torch.uint8).reshape(-1, w.shape[-1]).to(self.device)
             return self._maybe_dequant(QLinear("fp8", c.shape[0], c.shape[1], codes=c.contiguous(), row_scale=rs,
                                                experts=experts))
+        if w.dtype == torch.int8:
+            rs = self._t(stem + ".weight_scale").float().reshape(-1).to(self.device)
+            c = codec.rows16(w.reshape(-1, w.shape[-1]).to(self.device))
+            return self._maybe_dequant(QLinear("int8", c.shape[0], c.shape[1], codes=c, row_scale=rs))
         fmt = fmt_for(self.recipe, stem + suffix)
         w = w.to(self.device)
         fq = fmt_for(self.fake_quant, stem + suffix) if self.fake_quant is not None else "bf16"

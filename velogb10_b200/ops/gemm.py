@@ -101,6 +101,8 @@ def prepare(q: QLinear, keep_canonical: bool = True, splitk: Optional[int] = Non
     """Build (once) the tensor-core layout of a linear that lives on a CUDA device."""
     if q.kernel is not None:
         return q.kernel
+    if q.fmt == "int8":
+        raise _lib.KernelError("int8 weights are read in place: use int8.linear_int8")
     if q.fmt == "nvfp4":
         wt, fmt, rs = tile_nvfp4(q.packed, q.scales), WF_NVFP4, q.row_scale
     elif q.fmt == "fp8":
@@ -151,8 +153,8 @@ def linear_simt(q: QLinear, x16: torch.Tensor, n: Optional[int] = None, out: Opt
         w, sc = q.codes, None
     else:
         w, sc = q.w, None
-    if w is None:
-        raise _lib.KernelError("canonical weights were released; use linear()")
+    if w is None or q.fmt == "int8":
+        raise _lib.KernelError("canonical weights were released or are int8; use linear() / int8.linear_int8()")
     L = _lib.lib()
     rc = L.vg_gemm_simt(ptr(w), ptr(sc), ptr(q.row_scale), ptr(x16), ptr(out),
                         c_int(1 if out.dtype == torch.float32 else 0), c_int(q.m), c_int(q.k), c_int(n),

@@ -1,7 +1,8 @@
 """Quantization recipes: which tensor group is stored in which format.
 
 Grammar (reference: src/quant.rs:334-418): comma-separated tokens ``group[:fmt]`` or ``-group``;
-``fmt`` is ``nvfp4`` (default), ``fp8`` or ``bf16``; ``all`` expands to every group. Later tokens
+``fmt`` is ``nvfp4`` (default), ``fp8``, ``bf16`` or, for the dense groups ``mlp`` / ``attn`` / ``gdn`` only, ``int8``
+(8-bit weights and activations, not in the reference); ``all`` expands to every group. Later tokens
 override earlier ones. Examples: ``all`` (nvfp4-full), ``all,gdn:fp8`` (nvfp4-mixed),
 ``all,-router,-embed,-lmhead``.
 """
@@ -9,6 +10,7 @@ from __future__ import annotations
 
 from typing import Dict, Optional
 
+INT8_GROUPS = ("mlp", "attn", "gdn")
 GROUPS = ("mlp", "attn", "gdn", "lmhead", "embed", "mtp", "router", "expert")
 NAMED_RECIPES = {"nvfp4-full": "all", "nvfp4-mixed": "all,gdn:fp8", "gdn4": "all", "bf16": "off"}
 
@@ -49,7 +51,7 @@ def parse_recipe(spec: str) -> Optional[Dict[str, str]]:
             tok = tok[1:]
         name, _, fmt = tok.partition(":")
         fmt = fmt or "nvfp4"
-        if fmt not in ("nvfp4", "fp8", "bf16"):
+        if fmt not in ("nvfp4", "fp8", "int8", "bf16"):
             raise ValueError(f"unknown format {fmt!r} in recipe")
         if name == "all":
             groups = list(GROUPS)
@@ -57,6 +59,8 @@ def parse_recipe(spec: str) -> Optional[Dict[str, str]]:
             groups = [name]
         else:
             raise ValueError(f"unknown group {name!r} in recipe")
+        if fmt == "int8" and not neg and not set(groups) <= set(INT8_GROUPS):
+            raise ValueError(f"int8 is for the groups {', '.join(INT8_GROUPS)}, not {name!r}")
         for g in groups:
             out.pop(g, None)
             if not neg and fmt != "bf16":
