@@ -337,6 +337,42 @@ def test_product_into_views_leaves_the_rest_alone():
         assert torch.equal(I8.linear_int8(q2, act, n=n), I8.linear_int8(q, act, n=n))
 
 
+def test_first_call_may_not_be_captured(monkeypatch):
+    from velogb10_b200.ops import int8 as I8, lib
+    x = torch.zeros((1, 16), device="cuda")
+    monkeypatch.setattr(I8, "_devices", {})
+    monkeypatch.setattr(lib, "_err_words", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(lib.KernelError, match="before capturing"):
+        I8.quantize_act_int8(x)
+    monkeypatch.undo()
+    I8.quantize_act_int8(x)
+
+
+def test_calls_on_two_streams_at_once():
+    """Every form of the product and the quantisers in flight on two streams: nothing is shared between calls."""
+    from velogb10_b200.ops import int8 as I8, lib
+    jobs = []
+    for i, (m, k, n) in enumerate(((5120, 4160, 3), (640, 5120, 40), (1001, 2063, 203), (5120, 6144, 256), (5120, 1024, 1200))):
+        q, x = _weights(m, k, i), _randn((n, k), i, BF)
+        act = I8.quantize_act_int8(x)
+        jobs.append((q, x, act.q.clone(), act.scale.clone(), I8.linear_int8(q, act)))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for r in range(10):
+        for i, (q, x, *_) in enumerate(jobs):
+            with torch.cuda.stream(streams[(r + i) % 2]):
+                act = I8.quantize_act_int8(x)
+                got.append((i, act, I8.linear_int8(q, act)))
+    torch.cuda.synchronize()
+    lib.check_err_word()
+    for i, act, out in got:
+        _, _, codes, scale, want = jobs[i]
+        assert torch.equal(act.q, codes) and torch.equal(act.scale, scale) and torch.equal(out, want), i
+
+
 def test_no_rows():
     from velogb10_b200.ops import int8 as I8
     act = I8.quantize_act_int8(torch.zeros((0, 64), device="cuda"))

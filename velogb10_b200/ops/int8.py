@@ -63,6 +63,9 @@ def _fn(name: str):
 def _device(device: torch.device):
     if device.type != "cuda":
         raise KernelError(f"the 8-bit integer path runs on CUDA tensors, got {device}")
+    if torch.cuda.is_current_stream_capturing() and device not in _lib._err_words:
+        # made here, the word would be cleared by every replay instead of once
+        raise KernelError("call the 8-bit integer path once before capturing it: its error word does not exist yet")
     d = _devices[device] = (device.index, _lib.err_word(device).data_ptr())
     return d
 
