@@ -340,7 +340,7 @@ def test_product_into_views_leaves_the_rest_alone():
 def test_first_call_may_not_be_captured(monkeypatch):
     from velogb10_b200.ops import int8 as I8, lib
     x = torch.zeros((1, 16), device="cuda")
-    monkeypatch.setattr(I8, "_devices", {})
+    monkeypatch.setattr(I8, "_err", {})
     monkeypatch.setattr(lib, "_err_words", {})
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(lib.KernelError, match="before capturing"):

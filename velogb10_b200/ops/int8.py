@@ -49,7 +49,7 @@ _TYPES = {"vg_quant_int8": (_P, _L, _I, _I, _I, _P, _L, _P, _P, _P),
           "vg_dequant_int8": (_P, _L, _P, _P, _L, _I, _I, _I, _P, _P),
           "vg_gemm_int8": (_P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _P, _P)}
 _fns = {}
-_devices = {}                  # CUDA device -> (index, address of its error word)
+_err = {}                      # device index -> address of the device's error word
 
 
 def _fn(name: str):
@@ -60,19 +60,20 @@ def _fn(name: str):
     return f
 
 
-def _device(device: torch.device):
-    if device.type != "cuda":
-        raise KernelError(f"the 8-bit integer path runs on CUDA tensors, got {device}")
+def _err_word(index: int) -> int:
+    if index < 0:
+        raise KernelError("the 8-bit integer path runs on CUDA tensors")
+    device = torch.device("cuda", index)
     if torch.cuda.is_current_stream_capturing() and device not in _lib._err_words:
         # made here, the word would be cleared by every replay instead of once
         raise KernelError("call the 8-bit integer path once before capturing it: its error word does not exist yet")
-    d = _devices[device] = (device.index, _lib.err_word(device).data_ptr())
-    return d
+    p = _err[index] = _lib.err_word(device).data_ptr()
+    return p
 
 
-def _launch(name: str, device: torch.device, *args):
-    """Enqueues on the current stream of ``device``; every entry ends with (error word, stream)."""
-    index, err = _devices.get(device) or _device(device)
+def _launch(name: str, index: int, *args):
+    """Enqueues on the current stream of device ``index``; every entry ends with (error word, stream)."""
+    err = _err.get(index) or _err_word(index)
     fn = _fns.get(name) or _fn(name)
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
@@ -107,43 +108,45 @@ def _pitch(t: torch.Tensor, what: str, rows: int, cols: int) -> int:
     return ld if rows > 1 else max(ld, cols)
 
 
-def _matrix(t: torch.Tensor, what: str, dtypes, rows: int, cols: int, device) -> int:
+def _matrix(t: torch.Tensor, what: str, dtypes, rows: int, cols: int, index: int) -> int:
     """Row pitch of a 2-D row-major argument that has to hold ``rows`` x ``cols`` elements."""
     if t.dtype not in dtypes:
         raise KernelError(f"{what}: dtype {t.dtype} is not supported")
     shape = t.shape
     if len(shape) != 2 or shape[0] < rows or shape[1] != cols:
         raise KernelError(f"{what}: shape {tuple(shape)}, expected at least {rows} rows of {cols}")
-    if t.device != device:
-        raise KernelError(f"{what} is on {t.device}, expected {device}")
+    if t.get_device() != index:
+        raise KernelError(f"{what} is on {t.device}, expected CUDA device {index}")
     ld, inner = t.stride()
     return ld if inner == 1 and ld >= cols else _pitch(t, what, rows, cols)
 
 
-def _vector(t: torch.Tensor, what: str, size: int, device, least: bool = False):
-    if t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] < size or (t.shape[0] != size and not least) \
-            or t.device != device or not t.is_contiguous():
-        raise KernelError(f"{what}: expected {size} contiguous fp32 values on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _vector(t: torch.Tensor, what: str, size: int, index: int, least: bool = False):
+    shape = t.shape
+    if t.dtype is not torch.float32 or len(shape) != 1 or (shape[0] < size if least else shape[0] != size) \
+            or t.get_device() != index or not t.is_contiguous():
+        raise KernelError(f"{what}: expected {size} contiguous fp32 values on CUDA device {index}, "
+                          f"got {t.dtype} {tuple(shape)} on {t.device}")
 
 
-def _out(out: Optional[Int8Act], n: int, k: int, device):
+def _out(out: Optional[Int8Act], n: int, k: int, like: torch.Tensor):
     """The quantisers' output buffers and their row pitch."""
     if k < 1 or k > MAX_K:
         raise KernelError(f"row width {k} is outside 1 .. {MAX_K}")
     if out is None:
-        return act_buffers(n, k, device), (k + 15) & ~15
-    ld = _matrix(out.q, "out.q", _INT8, n, k, device)
-    _vector(out.scale, "out.scale", n, device, least=True)
+        return act_buffers(n, k, like.device), (k + 15) & ~15
+    index = like.get_device()
+    ld = _matrix(out.q, "out.q", _INT8, n, k, index)
+    _vector(out.scale, "out.scale", n, index, least=True)
     return out, ld
 
 
 def quantize_act_int8(x: torch.Tensor, n: Optional[int] = None, out: Optional[Int8Act] = None) -> Int8Act:
     """Quantise rows ``x[:n]`` (bf16 / f16 / f32 ``[rows, k]``)."""
     n, k, ld = _input(x, "x", _DTYPE, n)
-    dev = x.device
-    out, ldq = _out(out, n, k, dev)
+    out, ldq = _out(out, n, k, x)
     if n:
-        _launch("vg_quant_int8", dev, x.data_ptr(), ld, _DTYPE[x.dtype], n, k, out.q.data_ptr(), ldq, out.scale.data_ptr())
+        _launch("vg_quant_int8", x.get_device(), x.data_ptr(), ld, _DTYPE[x.dtype], n, k, out.q.data_ptr(), ldq, out.scale.data_ptr())
     return out
 
 
@@ -154,10 +157,9 @@ def swiglu_int8(gu: torch.Tensor, n: Optional[int] = None, inter: Optional[int] 
         inter = cols // 2
     if cols != 2 * inter:
         raise KernelError(f"gu: {cols} columns, expected 2 * {inter}")
-    dev = gu.device
-    out, ldq = _out(out, n, inter, dev)
+    out, ldq = _out(out, n, inter, gu)
     if n:
-        _launch("vg_swiglu_int8", dev, gu.data_ptr(), ld, n, inter, out.q.data_ptr(), ldq, out.scale.data_ptr())
+        _launch("vg_swiglu_int8", gu.get_device(), gu.data_ptr(), ld, n, inter, out.q.data_ptr(), ldq, out.scale.data_ptr())
     return out
 
 
@@ -166,10 +168,10 @@ def add_rmsnorm_int8(res: torch.Tensor, delta: Optional[torch.Tensor], w: torch.
     """``res[:n] += delta[:n]`` (bf16, in place, when delta is given), then RMSNorm with weights ``w`` (``1 + w`` with
     ``plus_one``) quantised; the normed rows also go to ``out16`` (f16, saturating) when it is given."""
     n, h, ld = _input(res, "res", _BF16, n)
-    dev = res.device
+    dev = res.get_device()
     if not eps > 0.0:
         raise KernelError(f"eps must be positive, got {eps}")
-    out, ldq = _out(out, n, h, dev)
+    out, ldq = _out(out, n, h, res)
     ldd = ldo = 0
     if delta is not None:
         ldd = _matrix(delta, "delta", _BF16, n, h, dev)
@@ -186,20 +188,21 @@ def add_rmsnorm_int8(res: torch.Tensor, delta: Optional[torch.Tensor], w: torch.
 def dequantize_act_int8(act: Int8Act, n: Optional[int] = None, out: Optional[torch.Tensor] = None,
                         dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values rows ``act.q[:n]`` stand for, in bf16, f16 (saturating) or f32 (``out``'s type when it is given)."""
-    n, k, ldq = _input(act.q, "act.q", _INT8, n)
-    dev = act.q.device
+    q = act.q
+    n, k, ldq = _input(q, "act.q", _INT8, n)
+    dev = q.get_device()
     if k < 1 or k > MAX_K:
         raise KernelError(f"row width {k} is outside 1 .. {MAX_K}")
     _vector(act.scale, "act.scale", n, dev, least=True)
     if out is None:
         if dtype not in _DTYPE:
             raise KernelError(f"dtype {dtype} is not supported")
-        out = torch.empty(n, k, dtype=dtype, device=dev)
+        out = torch.empty(n, k, dtype=dtype, device=q.device)
         ldo = k
     else:
         ldo = _matrix(out, "out", _DTYPE, n, k, dev)
     if n:
-        _launch("vg_dequant_int8", dev, act.q.data_ptr(), ldq, act.scale.data_ptr(), out.data_ptr(), ldo, _DTYPE[out.dtype], n, k)
+        _launch("vg_dequant_int8", dev, q.data_ptr(), ldq, act.scale.data_ptr(), out.data_ptr(), ldo, _DTYPE[out.dtype], n, k)
     return out
 
 
@@ -210,7 +213,7 @@ def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional
     if q.fmt != "int8":
         raise KernelError(f"linear_int8 takes int8 weights, got {q.fmt}")
     n, cols, ldq = _input(act.q, "act.q", _INT8, n)
-    m, k, dev = q.m, q.k, act.q.device
+    m, k, dev = q.m, q.k, act.q.get_device()
     if k < 1 or k > MAX_K or m < 1:
         raise KernelError(f"weights [{m}, {k}]: K must be in 1 .. {MAX_K}")
     if cols != k:
@@ -226,7 +229,7 @@ def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional
     _vector(q.row_scale, "row_scale", m, dev)
     _vector(act.scale, "act.scale", n, dev, least=True)
     if out is None:
-        out = torch.empty(n, m, dtype=torch.float32 if out_f32 else torch.bfloat16, device=dev)
+        out = torch.empty(n, m, dtype=torch.float32 if out_f32 else torch.bfloat16, device=act.q.device)
         ldo = m
     else:
         ldo = _matrix(out, "out", (torch.bfloat16, torch.float32), n, m, dev)
