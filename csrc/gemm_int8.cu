@@ -75,7 +75,7 @@ struct OutWarp {
   VG_DEVINL OutWarp(const I8Params& p, int m, int n0) {
     const int lane = threadIdx.x & 31, es = p.out_f32 ? 4 : 2;
     pitch = (size_t)p.ldo * es;
-    sw = m < p.M ? __ldg(p.sw + m) : 0.f;
+    sw = m < p.M ? p.sw[m] : 0.f;
     in = m < p.M;           // vec needs M % 4 == 0: the four channels are inside or outside together
     base = static_cast<char*>(p.out) + (p.vec ? (size_t)(n0 + (lane & 3)) * pitch + (size_t)(m & ~3) * es
                                               : (size_t)n0 * pitch + (size_t)m * es);
@@ -175,7 +175,7 @@ VG_DEVINL void store_tile(const I8Params& p, const OutWarp& o, uint32_t acc, int
 // A warp's own copy of the token scales, fetched while the accumulator is still being built.
 VG_DEVINL void fetch_sx(const I8Params& p, float* sx, int n0, int cols) {
   __syncwarp();
-  for (int c = threadIdx.x & 31; c < (cols + 31) / 32 * 32; c += 32) sx[c] = c < cols ? __ldg(p.sx + n0 + c) : 0.f;
+  for (int c = threadIdx.x & 31; c < (cols + 31) / 32 * 32; c += 32) sx[c] = c < cols ? p.sx[n0 + c] : 0.f;
   __syncwarp();
 }
 
@@ -660,7 +660,8 @@ const Room* room_of(int dev) {
 // Fitted to single rounds of 20 - 60 tiles at K = 6144 and 17408: a slab takes 0.157 us at 64 tokens (waiting and copying),
 // 0.19 at 128, 0.30 at 256 (MMAs: 512 cycles and the epilogue's share); a launch 3.6 us and 6 ns a token of its tiles,
 // 5 us more when partial sums travel. Splitting pays where there are few tiles and much K: 256 x 5120 x 17408 46.0 us
-// whole with 256-token tiles, 28.6 with 96, 26.7 split three ways; at K = 6144 12.9 with 96, 16.3 split.
+// whole with 256-token tiles, 28.6 with 96, 26.7 split three ways; at K = 6144 12.9 with 96, 16.3 split. Work and weight
+// stream overlap, but not fully (128 x 34816 x 5120: 32.9 us in one token tile, 39 in two).
 void choose_pair(int N, int K, int M, const Room& room, PairShape* sh, int* split) {
   const int slabs = (K + BK - 1) / BK, least = (N + PBN - 1) / PBN;
   const double weights = (double)M * K / 6.2e6;                 // from memory at 6.2 TB/s
@@ -673,7 +674,7 @@ void choose_pair(int N, int K, int M, const Room& room, PairShape* sh, int* spli
     for (int s = 1; s <= PAIR_MAX_SPLIT && s <= max(1, slabs / 4); ++s) {
       const double rounds = ceil((double)sh->tiles.mt * used / max(1, room.clusters[2 * s]));
       const double work = rounds * ((slabs + s - 1) / s) * slab, fixed = 3.6 + 0.006 * bn;
-      const double t = max(work, weights) + (s > 1 ? rounds * (fixed + 4.0 + 0.5 * s) : fixed);
+      const double t = max(work, weights) + 0.2 * min(work, weights) + (s > 1 ? rounds * (fixed + 4.0 + 0.5 * s) : fixed);
       if (t < best) {
         best = t;
         sh->bn = bn;

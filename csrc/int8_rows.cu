@@ -11,6 +11,8 @@
 // inputs and outputs once and nothing else. A row that holds an infinity or a NaN (or whose sum of squares leaves
 // fp32) gets scale NaN and codes 0: everything computed from it is NaN instead of a plausible wrong number. The floor
 // of the scale keeps an all-zero row at codes 0 and 1 / s finite.
+// Inputs are read with ordinary loads: a kernel may start before its predecessor has written them, so they are not
+// read-only for its lifetime, which ld.global.nc (restrict pointers, __ldg) asks for.
 #include <atomic>
 
 #include "common.cuh"
@@ -405,7 +407,7 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
           unpack8(r4, v[c], false);
         }
         if (KIND == ROW_NORM) {
-          const float4 w0 = __ldg(reinterpret_cast<const float4*>(p.w + e)), w1 = __ldg(reinterpret_cast<const float4*>(p.w + e + 4));
+          const float4 w0 = *reinterpret_cast<const float4*>(p.w + e), w1 = *reinterpret_cast<const float4*>(p.w + e + 4);
           const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -462,8 +464,8 @@ VG_DEVINL void dequant4(uint32_t c, float s, OUT* o) {
   for (int i = 0; i < 4; ++i) o[i] = from_f32<OUT>((float)(signed char)(c >> (8 * i)) * s);
 }
 template <typename OUT, int R>
-__global__ void __launch_bounds__(1024) dequant_int8_kernel(const signed char* __restrict__ q, long long ldq,
-                                                            const float* __restrict__ scale, OUT* __restrict__ out,
+__global__ void __launch_bounds__(1024) dequant_int8_kernel(const signed char* q, long long ldq,
+                                                            const float* scale, OUT* out,
                                                             long long ldo, int n, int k) {
   pdl_trigger();
   pdl_wait();
@@ -493,8 +495,8 @@ __global__ void __launch_bounds__(1024) dequant_int8_kernel(const signed char* _
 // Any width and pitch: groups of eight that start on the output's 16-byte boundaries; their codes come from the two
 // aligned words around them where those lie inside the row.
 template <typename OUT>
-__global__ void __launch_bounds__(256) dequant_int8_loose_kernel(const signed char* __restrict__ q, long long ldq,
-                                                                 const float* __restrict__ scale, OUT* __restrict__ out,
+__global__ void __launch_bounds__(256) dequant_int8_loose_kernel(const signed char* q, long long ldq,
+                                                                 const float* scale, OUT* out,
                                                                  long long ldo, int k) {
   pdl_trigger();
   pdl_wait();

@@ -77,6 +77,28 @@ def test_recipe_and_checkpoint(tmp_path):
     assert n == 2 * cfg.num_layers + 2 * cfg.num_layers          # mixer in / out and MLP in / down of every layer
 
 
+def test_int8_tensors_without_int8_kernels_load_as_bf16():
+    from velogb10_b200.config import tiny_hybrid
+    from velogb10_b200.models.weights import ModelBuilder
+    g = torch.Generator().manual_seed(0)
+    two, three = torch.randn(32, 48, generator=g), torch.randn(4, 16, 32, generator=g)
+    a, b = codec.quantize_int8(two), codec.quantize_int8(three.reshape(64, 32))
+    tensors = {"lm_head.weight": a.codes, "lm_head.weight_scale": a.row_scale,
+               "layers.0.mlp.experts.gate_up_proj": b.codes.reshape(4, 16, 32),
+               "layers.0.mlp.experts.gate_up_proj.weight_scale": b.row_scale.reshape(4, 16),
+               "layers.0.mlp.up_proj.weight": a.codes, "layers.0.mlp.up_proj.weight_scale": a.row_scale[:, None]}
+
+    class Source:
+        def get(self, name):
+            return tensors.get(name)
+
+    mb = ModelBuilder(tiny_hybrid(False), Source())
+    head, experts, up = mb.linear("lm_head"), mb.linear("layers.0.mlp.experts.gate_up_proj", ""), mb.linear("layers.0.mlp.up_proj")
+    assert head.fmt == "bf16" and torch.equal(head.w, codec.dequantize_int8(a.codes, a.row_scale))
+    assert experts.fmt == "bf16" and experts.experts == 4 and torch.equal(experts.w, codec.dequantize_int8(b.codes, b.row_scale))
+    assert up.fmt == "int8" and torch.equal(up.codes, a.codes) and torch.equal(up.row_scale, a.row_scale)
+
+
 def test_other_linears_refuse_int8_weights():
     from velogb10_b200.ops import gemm as G
     q = _w(16, 32)

@@ -26,7 +26,7 @@ import torch
 
 from ..config import ModelConfig
 from ..quant import codec
-from ..quant.recipe import fmt_for, parse_recipe
+from ..quant.recipe import INT8_GROUPS, fmt_for, group_of, parse_recipe
 
 
 @dataclass
@@ -360,6 +360,9 @@ class ModelBuilder:
                                                experts=experts))
         if w.dtype == torch.int8:
             rs = self._t(stem + ".weight_scale").float().reshape(-1).to(self.device)
+            if w.dim() == 3 or group_of(stem + suffix) not in INT8_GROUPS:       # no int8 kernels for these: bf16
+                dense = w.to(self.device).float() * rs.reshape(w.shape[:-1]).unsqueeze(-1)
+                return QLinear.from_dense(dense.to(torch.bfloat16), "bf16")
             c = codec.rows16(w.reshape(-1, w.shape[-1]).to(self.device))
             return self._maybe_dequant(QLinear("int8", c.shape[0], c.shape[1], codes=c, row_scale=rs))
         fmt = fmt_for(self.recipe, stem + suffix)
