@@ -36,9 +36,11 @@ class Int8Act:
 
 def act_buffers(rows: int, k: int, device) -> Int8Act:
     """Buffers a quantiser can write into (``out=``) and ``linear_int8`` can read."""
-    kp = (k + 15) & ~15
-    q = torch.empty(rows, kp, dtype=torch.int8, device=device)
-    return Int8Act(q if kp == k else q[:, :k], torch.empty(rows, dtype=torch.float32, device=device))
+    if k & 15:
+        q = torch.empty_strided((rows, k), ((k + 15) & ~15, 1), dtype=torch.int8, device=device)
+    else:
+        q = torch.empty(rows, k, dtype=torch.int8, device=device)
+    return Int8Act(q, torch.empty(rows, dtype=torch.float32, device=device))
 
 
 # argument types of the C entries, set once so that plain ints and floats convert without wrapper objects
