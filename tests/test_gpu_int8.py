@@ -337,6 +337,52 @@ def test_product_into_views_leaves_the_rest_alone():
         assert torch.equal(I8.linear_int8(q2, act, n=n), I8.linear_int8(q, act, n=n))
 
 
+def _spread(t, pitch):
+    """The matrix with its rows `pitch` elements apart; what lies between is never touched."""
+    buf = torch.empty((t.shape[0] - 1) * pitch + t.shape[1], dtype=t.dtype, device="cuda")
+    view = buf.as_strided(t.shape, (pitch, 1))
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("n,k,pitch", [(3, 264, (1 << 30) + 64), (3, 263, (1 << 30) + 48), (1200, 264, 1800016)])
+def test_offsets_past_32_bits(n, k, pitch):
+    """Rows that start more than 2^31 elements into their buffer, few of them and many: the bits of near rows. These start
+    at the same places within 16 bytes, since the order of the norm's sum goes by that."""
+    from velogb10_b200.ops import int8 as I8
+    assert (n - 1) * pitch > 1 << 31 and pitch % 16 == 0
+    far, near = (lambda t: _spread(t, pitch)), (lambda t: _spread(t, 1072))
+    x, d, gu, w = _randn((n, k), 1, BF), _randn((n, k), 3, BF), _randn((n, 2 * k), 2, BF), _randn((k,), 4)
+    got = []
+    for place in (far, near):
+        out = I8.Int8Act(place(torch.zeros((n, k), dtype=torch.int8, device="cuda")), torch.zeros(n, device="cuda"))
+        f16, res, r = place(torch.zeros((n, k), dtype=F16, device="cuda")), place(x), []
+        I8.quantize_act_int8(res, out=out)
+        r += [out.q.clone(), out.scale.clone()]
+        I8.dequantize_act_int8(out, out=f16)
+        r += [f16.clone()]
+        I8.swiglu_int8(place(gu), out=out)
+        r += [out.q.clone(), out.scale.clone()]
+        I8.add_rmsnorm_int8(res, place(d), w, 1e-6, out=out, out16=f16)
+        got.append(r + [out.q.clone(), out.scale.clone(), f16.clone(), res.clone()])
+    _check_rows(I8.Int8Act(got[0][0], got[0][1]), x.double(), n, 0.0, (n, k))
+    assert [torch.equal(a, b) for a, b in zip(*got)] == [True] * 9
+
+
+@pytest.mark.parametrize("m,k,n,pitch", [(136, 264, 3, (1 << 30) + 64), (264, 520, 70, (1 << 25) + 16), (200, 264, 1200, 1800016)])
+def test_product_offsets_past_32_bits(m, k, n, pitch):
+    """Tokens and results (and with three tokens weights too) that lie beyond 2^31 elements."""
+    from velogb10_b200.ops import int8 as I8
+    assert (n - 1) * pitch > 1 << 31
+    q, act = _weights(m, k, 5), _tokens(n, k, 6)
+    want = I8.linear_int8(q, act)
+    far = I8.Int8Act(_spread(act.q, pitch), act.scale)
+    out = _spread(torch.zeros_like(want), pitch)
+    wide = type(q)("int8", m, k, codes=_spread(q.codes, 1 << 24), row_scale=q.row_scale)
+    I8.linear_int8(wide, far, out=out)
+    assert torch.equal(out, want)
+
+
 def test_first_call_may_not_be_captured(monkeypatch):
     from velogb10_b200.ops import int8 as I8, lib
     x = torch.zeros((1, 16), device="cuda")
