@@ -19,7 +19,7 @@ import torch
 
 from ..models.weights import QLinear
 from . import lib as _lib
-from .lib import KernelError, c_float, c_int, c_ll, c_void_p
+from .lib import KernelError, c_float, c_int, c_ll, c_void_p, empty_beside as _empty
 
 MAX_K = 131071                 # 128 * 128 * K must stay below 2^31
 MAX_ROWS = 1 << 27
@@ -77,7 +77,7 @@ def _launch(name: str, index: int, *args):
     """Enqueues on the current stream of device ``index``; every entry ends with (error word, stream)."""
     err = _err.get(index) or _err_word(index)
     fn = _fns.get(name) or _fn(name)
-    if index != torch.cuda.current_device():
+    if index != _lib.current_index():
         with torch.cuda.device(index):
             _lib.check(fn(*args, err, _lib.raw_stream(index)), name)
         return
@@ -136,7 +136,8 @@ def _out(out: Optional[Int8Act], n: int, k: int, like: torch.Tensor):
     if k < 1 or k > MAX_K:
         raise KernelError(f"row width {k} is outside 1 .. {MAX_K}")
     if out is None:
-        return act_buffers(n, k, like.device), (k + 15) & ~15
+        ld = (k + 15) & ~15
+        return Int8Act(_empty(like, (n, k), (ld, 1), torch.int8), _empty(like, (n,), (1,), torch.float32)), ld
     index = like.get_device()
     ld = _matrix(out.q, "out.q", _INT8, n, k, index)
     _vector(out.scale, "out.scale", n, index, least=True)
@@ -199,7 +200,7 @@ def dequantize_act_int8(act: Int8Act, n: Optional[int] = None, out: Optional[tor
     if out is None:
         if dtype not in _DTYPE:
             raise KernelError(f"dtype {dtype} is not supported")
-        out = torch.empty(n, k, dtype=dtype, device=q.device)
+        out = _empty(q, (n, k), (k, 1), dtype)
         ldo = k
     else:
         ldo = _matrix(out, "out", _DTYPE, n, k, dev)
@@ -231,7 +232,7 @@ def linear_int8(q: QLinear, act: Int8Act, n: Optional[int] = None, out: Optional
     _vector(q.row_scale, "row_scale", m, dev)
     _vector(act.scale, "act.scale", n, dev, least=True)
     if out is None:
-        out = torch.empty(n, m, dtype=torch.float32 if out_f32 else torch.bfloat16, device=act.q.device)
+        out = _empty(act.q, (n, m), (m, 1), torch.float32 if out_f32 else torch.bfloat16)
         ldo = m
     else:
         ldo = _matrix(out, "out", (torch.bfloat16, torch.float32), n, m, dev)

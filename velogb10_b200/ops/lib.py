@@ -61,6 +61,18 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+current_index = torch._C._cuda_getDevice        # current device, without the lazy-initialisation check (0.1 us of 0.2)
+_empty_strided_cuda = torch._C._dynamo.guards._empty_strided_cuda
+
+
+def empty_beside(like: torch.Tensor, shape, strides, dtype: torch.dtype) -> torch.Tensor:
+    """Uninitialised tensor on ``like``'s device. On the current CUDA device by the call PyTorch's own compiled code makes,
+    which takes the same memory but skips argument parsing and dispatch: 0.8 us instead of 1.5."""
+    if like.is_cuda and like.get_device() == current_index():
+        return _empty_strided_cuda(shape, strides, dtype)
+    return torch.empty_strided(shape, strides, dtype=dtype, device=like.device)
+
+
 launches = 0        # kernels enqueued through this module since import (each wrapper reports its count)
 
 
