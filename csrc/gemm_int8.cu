@@ -180,7 +180,9 @@ VG_DEVINL void fetch_sx(const I8Params& p, float* sx, int n0, int cols) {
 }
 
 // Split K: columns go in groups of four, group g to the part g % parts. A part's receive area (over the drained ring)
-// holds [source part][own group][channel] as 16-byte words.
+// holds [source part][own group][channel] as 16-byte words. 64 x 5120 x 17408 in seven parts: sending takes 1.9 us and
+// joining 1.7 of 19.0; 256 tokens in three parts 2.9 and 3.4 of 26.7. Sending moves 15 bytes a cycle and SM between SMs
+// whatever the order of the parts, the columns read at a time (16, 32, 64) or the way the own part is kept.
 VG_DEVINL uint32_t group_slots(int cols, int parts) { return (uint32_t)(((cols + 3) / 4 + parts - 1) / parts); }
 // `to_rank(part)`: cluster rank of the CTA of that part which holds the same channels
 template <typename F>
