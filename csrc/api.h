@@ -93,7 +93,8 @@ int vg_gemm_tc_set_debug(int dbg, long long* trace_buf);   // profiling builds o
 int vg_gemm_simt(const void* wq, const void* scales, const float* row_scale, const void* x_f16, void* out, int out_f32,
                  int M, int K, int N, int ldx, int ldo, int wfmt, cudaStream_t stream);
 
-// 8-bit integer (W8A8) path. Rows y become int8 codes q = rint(y / s) with one fp32 scale s = max(max|y| / 127, 2^-120)
+// 8-bit integer (W8A8) path. Rows y become int8 codes q = rint(y / s) with one fp32 scale s = max(max|y| / 127, 2^-120),
+// half to even: vg_quant_int8 by the exact quotient 127 y / max|y|, the others, whose y are rounded themselves, by y * (1 / s)
 // (scale NaN and codes 0 for a row that holds an infinity or a NaN); k <= 131072. dtype: 0 bf16, 1 f16, 2 f32.
 // vg_gemm_int8: out[n, m] = (sum_k q[n, k] codes[m, k]) * sx[n] * sw[m]; K <= 131071, code rows on 16-byte boundaries.
 int vg_quant_int8(const void* x, long long ldx, int dtype, int n, int k, void* q, long long ldq, float* scale,

@@ -2,6 +2,10 @@
 //
 //   s = max(max_k |y_k| / 127, 2^-120),   q_k = rint(y_k / s)   (half to even, |q| <= 127)
 //
+// For rows that are read (vg_quant_int8) q is that of the exact quotient 127 y / max|y|, so that no rounding decides a code.
+// For rows that are computed here y has rounding errors of its own, and q is rint(y * (1 / s)), which may differ from
+// rint(y / s) where y / s is within 2^-16 of a half.
+//
 //   vg_quant_int8         y = x                                       (bf16 / f16 / f32 rows)
 //   vg_add_rmsnorm_int8   res += delta;  y = res * rsqrt(mean res^2 + eps) * (w [+ 1])
 //   vg_swiglu_int8        y = silu(gate) * up
@@ -24,7 +28,10 @@ using namespace vg;
 constexpr int MAX_CLUSTER = 8;
 constexpr int RING_SLOTS = 8;
 constexpr float INT8_MAX_CODE = 127.0f;
-constexpr float SCALE_FLOOR = 7.52316384526264e-37f;      // 2^-120
+constexpr float AMAX_FLOOR = 127.0f * 0x1p-120f;          // exact; its scale is 2^-120
+constexpr float BIG_ROW = 0x1p100f, SHRINK = 0x1p-64f;
+constexpr float ROUND_MAGIC = 12582912.0f;                // 1.5 * 2^23
+constexpr float NEAR_HALF = 0.5f - 0x1p-15f;
 
 enum RowKind { ROW_BF16 = 0, ROW_F16 = 1, ROW_F32 = 2, ROW_SWIGLU = 3, ROW_NORM = 4 };
 
@@ -67,15 +74,6 @@ VG_DEVINL void block_reduce(unsigned& mx, float& sum, unsigned* red_m, float* re
   if (SUM) sum = warp_sum(lane < nw ? red_s[lane] : 0.f);
 }
 
-// Eight values -> eight codes, rint(v * f) for |v * f| < 2^22: adding 1.5 * 2^23 leaves the rounded integer in the low bits
-// of the sum. (cvt.rni runs at an eighth of the rate, next to the exponentials.)
-VG_DEVINL uint2 codes8(const float* v, float f) {
-  uint32_t t[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = __float_as_uint(__fmaf_rn(v[i], f, 12582912.0f));
-  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
-                    __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
-}
 VG_DEVINL void unpack8(uint4 a, float* v, bool f16) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -105,9 +103,10 @@ VG_DEVINL uint4 pack_f16_sat(const float* v) {
   return o;
 }
 
-// What a row's statistics give: the scale, its reciprocal and (norm) 1 / rms.
+// What a row's statistics give: the largest value, the scale, the factor from value to code in two terms (the second for
+// 16-bit rows only) and (norm) 1 / rms.
 struct RowScale {
-  float s, f, inv;
+  float amax, s, f, f_lo, inv;
   bool bad;
 };
 template <int KIND>
@@ -118,10 +117,77 @@ VG_DEVINL RowScale row_scale(const RowParams& p, unsigned mx, float ss) {
   o.inv = KIND == ROW_NORM ? rsqrtf(ss / (float)p.k + p.eps) : 1.f;
   const float amax = __uint_as_float(mx) * o.inv;
   o.bad = !(amax < INFINITY) || (KIND == ROW_NORM && !(ss < INFINITY));
-  o.s = o.bad ? __uint_as_float(0x7fffffffu) : fmaxf(__fdiv_rn(amax, INT8_MAX_CODE), SCALE_FLOOR);
-  // codes are rint(y * (1 / s)): |y| / s <= 127 (1 + 2^-22), which rounds to 127 at most; 1 / s <= 2^120
-  o.f = o.bad ? 0.f : __fdiv_rn(1.f, o.s);
+  o.amax = fmaxf(amax, AMAX_FLOOR);
+  o.s = o.bad ? __uint_as_float(0x7fffffffu) : __fdiv_rn(o.amax, INT8_MAX_CODE);       // 2^-120 or more, so 1 / s <= 2^120
+  if (KIND == ROW_BF16 || KIND == ROW_F16) {
+    if (o.amax > BIG_ROW) o.amax *= SHRINK;                       // so that f_lo does not underflow; the values follow
+    o.f = o.bad ? 0.f : __fdiv_rn(INT8_MAX_CODE, o.amax);
+    o.f_lo = __fmaf_rn(-o.f, o.amax, INT8_MAX_CODE) * o.f * (1.f / INT8_MAX_CODE);      // exact remainder / amax
+  } else {
+    o.f = o.bad ? 0.f : __fdiv_rn(1.f, o.s);
+    o.f_lo = 0.f;
+  }
   return o;
+}
+
+// Code of one value: rint(127 v / amax), half to even, decided exactly. v * f is within 127.5 * 2^-23 < 2^-16 of 127 v / amax,
+// so the code is the integer next to it or, close to a half, the one beyond the half. Which one, the sign of
+// 127 v - half * amax says: both products' leading 24 bits cancel, and what is left of each is exact in fp32 (scaled by a power
+// of two, so that nothing leaves its range).
+VG_DEVINL uint32_t code_near_half(float v, float f, float amax) {
+  const float m = __fmaf_rn(v, f, ROUND_MAGIC), n = m - ROUND_MAGIC, d = __fmaf_rn(v, f, -n);
+  if (!(fabsf(d) > NEAR_HALF)) return __float_as_uint(m);
+  const float out = copysignf(1.0f, d), half = n + 0.5f * out;    // the neighbour is n + out
+  const float unit = amax >= 1.0f ? 0x1p-10f : 0x1p100f, a = amax * unit;
+  const float p = half * a, low = __fmaf_rn(half, a, -p);
+  const float beyond = out * (__fmaf_rn(INT8_MAX_CODE, v * unit, -p) - low);
+  const bool odd = __float_as_uint(m) & 1;
+  return __float_as_uint(beyond > 0.f || (beyond == 0.f && odd) ? m + out : m);
+}
+// Eight values -> eight codes. Adding 1.5 * 2^23 leaves the rounded integer in the low bits of the sum. (cvt.rni runs at an
+// eighth of the rate, next to the exponentials.)
+// 16-bit rows hold many exact halves (127 v / amax = n + 1/2: one value in 6000 of a Gaussian bf16 row, every second one where
+// amax is 254 times a power of two); any other quotient is 2^-20 of its size or more away from a half, since v and amax have
+// 11 bits at most. v f + v f_lo, rounded twice, is off by 2^-23 at most, and for a half exactly right: the first product's
+// rounding is at most half a step, which the second rounding takes back. (4096 x 17408 bf16: one product 34.4 us, two
+// terms 38.3; 4096 x 5120 14.0 and 14.9. A test for halves and a branch, as below: 56, the rows above being the slow ones.)
+// fp32 rows can come closer to a half than any such sum: what is near one is decided by code_near_half (4096 x 5120: 20.0
+// without, 20.9 with).
+template <int KIND>
+VG_DEVINL uint2 codes8(const float* v, const RowScale& rs) {
+  uint32_t t[8];
+  if constexpr (KIND == ROW_BF16 || KIND == ROW_F16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = __float_as_uint(__fadd_rn(__fmaf_rn(v[i], rs.f_lo, __fmul_rn(v[i], rs.f)), ROUND_MAGIC));
+  } else if constexpr (KIND == ROW_F32) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float m0 = __fmaf_rn(v[i], rs.f, ROUND_MAGIC), m1 = __fmaf_rn(v[i + 1], rs.f, ROUND_MAGIC);
+      t[i] = __float_as_uint(m0);
+      t[i + 1] = __float_as_uint(m1);
+      most = max_abs3(most, __fmaf_rn(v[i], rs.f, ROUND_MAGIC - m0), __fmaf_rn(v[i + 1], rs.f, ROUND_MAGIC - m1));
+    }
+    if (most > NEAR_HALF) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = code_near_half(v[i], rs.f, rs.amax);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = __float_as_uint(__fmaf_rn(v[i], rs.f, ROUND_MAGIC));
+  }
+  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
+}
+// bf16 rows whose largest value is near the end of the range: see row_scale
+template <int KIND, int MAXC>
+VG_DEVINL void shrink_big_row(float (&v)[MAXC][8], unsigned mx) {
+  if (KIND == ROW_BF16 && __uint_as_float(mx) > BIG_ROW) {
+#pragma unroll
+    for (int c = 0; c < MAXC; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[c][i] *= SHRINK;
+  }
 }
 
 // Eight elements from element e of a row that starts at `base` and has `limit` of them in memory, as packed words; those
@@ -296,6 +362,7 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
   }
 
   const RowScale rs = row_scale<KIND>(p, mx, ss);
+  shrink_big_row<KIND>(v, mx);
   if (tid == 0) p.scale[row] = rs.s;
   if (KIND == ROW_NORM) {
 #pragma unroll
@@ -307,7 +374,7 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
 #pragma unroll
   for (int c = 0; c < MAXC; ++c) {
     const int e = e0 + c * e_step;
-    const uint2 codes = rs.bad ? make_uint2(0u, 0u) : codes8(v[c], rs.f);
+    const uint2 codes = rs.bad ? make_uint2(0u, 0u) : codes8<KIND>(v[c], rs);
     if (!VEC) store_codes_shifted(p.q + row * p.ldq, e, k, shift, codes);
     if (e < k && owner) {
       if (VEC) *reinterpret_cast<uint2*>(p.q + row * p.ldq + e) = codes;
@@ -427,6 +494,7 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
     if (stuck[team]) break;                                // seen by the whole team: set before the barrier
     if (tid == 0 && row + (long long)slots * step < n) fill(slot, j + slots, row + (size_t)slots * step);
     const RowScale rs = row_scale<KIND>(p, mx, ss);
+    shrink_big_row<KIND>(v, mx);
     if (tid == 0) p.scale[row] = rs.s;
 #pragma unroll
     for (int c = 0; c < MAXC; ++c) {
@@ -436,7 +504,7 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[c][i] *= rs.inv;
         }
-        *reinterpret_cast<uint2*>(p.q + (size_t)row * p.ldq + e) = rs.bad ? make_uint2(0u, 0u) : codes8(v[c], rs.f);
+        *reinterpret_cast<uint2*>(p.q + (size_t)row * p.ldq + e) = rs.bad ? make_uint2(0u, 0u) : codes8<KIND>(v[c], rs);
         if (KIND == ROW_NORM && p.out16) {
           const uint4 nan4 = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
           *reinterpret_cast<uint4*>(p.out16 + (size_t)row * p.ldo + e) = rs.bad ? nan4 : pack_f16_sat(v[c]);

@@ -484,3 +484,66 @@ def test_feed_forward_block(n, h, inter):
     res5 = res0 * 2
     assert torch.equal(out4, _block(res5, delta, w, gate_up, down)) and torch.equal(res4, res5)
     lib.check_err_word()
+
+
+def _exact_codes(y):
+    """rint(127 y / max|y|), half to even: in 64 bits the product is exact, and a quotient of 24-bit numbers that is not a half
+    lies 2^-33 or more of its size away from one."""
+    amax = y.double().abs().amax(-1, keepdim=True).clamp_min(127 * FLOOR)
+    return torch.round(y.double() * 127 / amax).to(torch.int8), (amax / torch.full_like(amax, 127.0)).float().squeeze(-1)
+
+
+# row form (whole words, shifted, two groups a thread, clusters) and ring form (several blocks an SM, one)
+@pytest.mark.parametrize("n,k", [(64, 6144), (64, 4111), (700, 4111), (9, 20000), (9, 17411), (1300, 512), (1200, 5120), (333, 17408)])
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+def test_exact_halves_round_to_even(n, k, dtype):
+    from velogb10_b200.ops import int8 as I8
+    from velogb10_b200.quant import codec
+    x = _randn((n, k), 3 * n + k, BF).to(dtype)                     # bf16 values in every type: halves are frequent
+    ratio = x.double() * 254 / x.double().abs().amax(-1, keepdim=True)
+    assert ((ratio == ratio.round()) & (ratio % 2 == 1)).sum() > n * k // 50000
+    act = I8.quantize_act_int8(x)
+    codes, scale = _exact_codes(x)
+    assert torch.equal(act.scale, scale)
+    assert torch.equal(act.q, codes)
+    q = codec.quantize_int8(x)                                      # weight rows: the same rule
+    assert torch.equal(q.codes, codes) and torch.equal(q.row_scale, scale)
+
+
+def test_codes_next_to_a_half_are_decided_exactly():
+    """fp32 values at a half and one and two fp32 steps beside it, for every code and several largest values; tiny rows at the
+    floor of the scale and rows near the end of fp32 among them."""
+    from velogb10_b200.ops import int8 as I8
+    h = torch.arange(-127, 127, dtype=F64, device="cuda") + 0.5
+    rows = []
+    for amax in (1.0, 127.0, 1.9999999, 3.3e38, 0.7, 1e-30, 2.0 ** -100, 127 * FLOOR, 3 * 127 * FLOOR / 4):
+        a = torch.tensor(amax, dtype=F32, device="cuda")
+        y = (h * a.double().clamp_min(127 * FLOOR) / 127).float()
+        near = [y]
+        for way in (float("inf"), -float("inf")):
+            b = y
+            for _ in range(2):
+                b = torch.nextafter(b, torch.full_like(b, way))
+                near.append(b)
+        t = torch.cat(near).clamp(-a, a)
+        rows.append(torch.cat([t, a[None]]))
+    x = torch.stack(rows)
+    codes, scale = _exact_codes(x)
+    for w in (x, torch.cat([x, torch.zeros_like(x)], 1)[:, :x.shape[1] + 1].contiguous()):
+        act = I8.quantize_act_int8(w)
+        assert torch.equal(act.scale, scale)
+        assert torch.equal(act.q[:, :x.shape[1]], codes)
+
+
+@pytest.mark.parametrize("dtype,bits,exps", [(BF, 8, (-110, -3, 99, 110, 120)), (F16, 11, (-14, 4))])
+def test_every_pair_of_16_bit_significands(dtype, bits, exps):
+    """All values whose code is not 0, against all largest values: exact quotients, exact halves, rows near the end of the range."""
+    from velogb10_b200.ops import int8 as I8
+    sig = torch.arange(1 << (bits - 1), 1 << bits, dtype=F64, device="cuda")
+    vals = torch.cat([sig * 2.0 ** -e for e in range(9)])
+    vals = torch.cat([vals, -vals])
+    for exp in exps:
+        x = (vals[None, :] * 2.0 ** (exp - bits + 1) * (vals.abs()[None, :] <= sig[:, None])).to(dtype)     # f16: subnormals among them
+        act = I8.quantize_act_int8(x)
+        codes, scale = _exact_codes(x)
+        assert torch.equal(act.scale, scale) and torch.equal(act.q, codes), exp

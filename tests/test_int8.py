@@ -170,3 +170,21 @@ BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 def test_refusals(what, call):
     with pytest.raises(KernelError, match=what):
         call()
+
+
+def test_codec_rounds_exact_halves_to_even():
+    """bf16 rows hold exact halves (127 w / max = n + 1/2), which a quotient of rounded numbers puts on either side. The rule
+    is checked in whole numbers: every bf16 value here is an integer times 2^-20."""
+    g = torch.Generator().manual_seed(7)
+    w = (torch.randn(40, 4001, generator=g) * 0.9).clamp(-7, 7).bfloat16()
+    w = torch.where(w.abs() < 2.0 ** -12, torch.zeros_like(w), w)
+    q = codec.quantize_int8(w)
+    v = (w.double() * 2 ** 20).long()
+    assert torch.equal(v.double() * 2.0 ** -20, w.double())
+    amax = v.abs().amax(-1, keepdim=True)
+    twice, rem = (254 * v.abs()) // amax, (254 * v.abs()) % amax           # quotient in half steps
+    half = (twice % 2 == 1) & (rem == 0)
+    want = torch.where(half, (twice // 2 + 1) // 2 * 2, (twice + 1) // 2) * v.sign()
+    assert half.sum() > 20
+    assert torch.equal(q.codes.long(), want)
+    assert torch.equal(q.row_scale, (amax.squeeze(-1).double() * 2.0 ** -20 / 127).float())

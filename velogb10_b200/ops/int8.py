@@ -1,7 +1,9 @@
 """The 8-bit integer (W8A8) linear path: row quantisers that feed it and the integer matrix product.
 
-A token row ``y`` becomes int8 codes with one fp32 scale, ``s = max(max|y| / 127, 2^-120)``, ``q = rint(y / s)``; a weight
-row (output channel) likewise, once, at load (``codec.quantize_int8``, ``QLinear.from_dense(w, "int8")``). The product
+A token row ``y`` becomes int8 codes with one fp32 scale, ``s = max(max|y| / 127, 2^-120)``, ``q = rint(y / s)``, half to even.
+``quantize_act_int8`` rounds the exact quotient ``127 y / max|y|``; the norm and SwiGLU, whose ``y`` are rounded fp32 values,
+round ``y * (1 / s)``, which is within 2^-16 of ``y / s``. A weight row (output channel) is quantised by the exact quotient
+too, once, at load (``codec.quantize_int8``, ``QLinear.from_dense(w, "int8")``). The product
 ``out[i, m] = (sum_k q[i, k] c[m, k]) * s[i] * row_scale[m]`` has an exact integer sum, so it depends neither on the batch
 width nor on how the kernel splits K.
 
