@@ -27,6 +27,9 @@ using namespace vg;
 
 constexpr int MAX_CLUSTER = 8;
 constexpr int RING_SLOTS = 8;
+constexpr int RING_GROUPS = 2560;                         // groups of eight of the widest row of the ring form
+// Largest row width: a cluster of eight CTAs of 1024 threads with two (three) groups of eight each.
+constexpr int ROW_MAX = MAX_CLUSTER * 1024 * 2 * 8;
 constexpr float INT8_MAX_CODE = 127.0f;
 constexpr float AMAX_FLOOR = 127.0f * 0x1p-120f;          // exact; its scale is 2^-120
 constexpr float BIG_ROW = 0x1p100f, SHRINK = 0x1p-64f;
@@ -44,7 +47,7 @@ struct RowParams {
   float* scale;
   __half* out16;                 // norm only, may be null
   int k, cluster;
-  float eps, w_off;
+  float eps, w_off, inv_k;       // norm only; inv_k = 1 / k
   int* err;
 };
 
@@ -54,24 +57,67 @@ VG_DEVINL float max_abs3(float m, float a, float b) {
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
   return r;
 }
-VG_DEVINL void dsmem_st_f32x2(uint32_t addr, float a, float b) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
+VG_DEVINL void dsmem_st_u32(uint32_t addr, unsigned v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// Maximum of a non-negative float's bits (so NaN > inf > finite) and sum over `threads` threads of which this is number
-// `tid`, one barrier: the block's, or named barrier `bar` of a team.
-template <bool SUM>
-VG_DEVINL void block_reduce(unsigned& mx, float& sum, unsigned* red_m, float* red_s, int tid, int threads, int bar = 0) {
+// The sum of a norm row's squares has one order whatever form runs the row, where it lies and how many rows there are, so a
+// token's codes do not depend on the batch: groups of eight consecutive elements one after the other, blocks of 32 groups
+// (256 elements, the lanes of a warp) by a butterfly, blocks i, i + 32, i + 64 .. by lane i, and another butterfly.
+constexpr int SUM_BLOCK = 256;
+// One butterfly for a warp's MAXC sums: the first steps halve the number of sums a lane carries along with the lanes that
+// carry each, so every sum is added in the order of warp_sum. Returns the sum of number `sum_of_lane`.
+template <int MAXC>
+VG_DEVINL int sum_of_lane(int lane) {
+  return MAXC == 1 ? 0 : MAXC == 2 ? lane >> 4 : lane >> 3;
+}
+template <int MAXC>
+VG_DEVINL float warp_sums(float (&s)[MAXC]) {
+  static_assert(MAXC == 1 || MAXC == 2 || MAXC == 4, "");
+  const int lane = threadIdx.x & 31;
+  float v = s[0];
+  if constexpr (MAXC == 1) {
+    v += __shfl_xor_sync(0xffffffffu, v, 16);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+  } else if constexpr (MAXC == 2) {
+    const bool hi = lane & 16;
+    v = (hi ? s[1] : s[0]) + __shfl_xor_sync(0xffffffffu, hi ? s[0] : s[1], 16);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+  } else {
+    const bool hi = lane & 16, second = lane & 8;
+    const float a = (hi ? s[2] : s[0]) + __shfl_xor_sync(0xffffffffu, hi ? s[0] : s[2], 16);
+    const float b = (hi ? s[3] : s[1]) + __shfl_xor_sync(0xffffffffu, hi ? s[1] : s[3], 16);
+    v = (second ? b : a) + __shfl_xor_sync(0xffffffffu, second ? a : b, 8);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// `blocks` <= 32 * MOST
+template <int MOST>
+VG_DEVINL float sum_of_blocks(const float* block, int blocks) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) {
+    const int i = (threadIdx.x & 31) + 32 * j;
+    s += i < blocks ? block[i] : 0.f;
+  }
+  return warp_sum(s);
+}
+
+// Over `threads` threads of which this is number `tid`, with one barrier (the block's, or named barrier `bar` of a team): the
+// maximum of a non-negative float's bits (so NaN > inf > finite), and (SUM) each warp's MAXC block sums to `block`.
+template <bool SUM, int MAXC>
+VG_DEVINL void block_reduce(unsigned& mx, float (&ss)[MAXC], unsigned* red_m, float* block, int tid, int threads, int bar = 0) {
   const int lane = tid & 31, w = tid >> 5, nw = threads >> 5;
   mx = __reduce_max_sync(0xffffffffu, mx);
-  if (SUM) sum = warp_sum(sum);
-  if (lane == 0) {
-    red_m[w] = mx;
-    if (SUM) red_s[w] = sum;
+  if constexpr (SUM) {
+    const float sum = warp_sums(ss);
+    if (lane % (32 / MAXC) == 0) block[w + sum_of_lane<MAXC>(lane) * nw] = sum;
   }
+  if (lane == 0) red_m[w] = mx;
   asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory");
   mx = __reduce_max_sync(0xffffffffu, lane < nw ? red_m[lane] : 0u);
-  if (SUM) sum = warp_sum(lane < nw ? red_s[lane] : 0.f);
 }
 
 VG_DEVINL void unpack8(uint4 a, float* v, bool f16) {
@@ -114,7 +160,7 @@ VG_DEVINL RowScale row_scale(const RowParams& p, unsigned mx, float ss) {
   // The norm's factor 1 / rms is common to the row, so the maximum of |res * w| found in the same pass as the sum of
   // squares is enough: one reduction instead of two.
   RowScale o;
-  o.inv = KIND == ROW_NORM ? rsqrtf(ss / (float)p.k + p.eps) : 1.f;
+  o.inv = KIND == ROW_NORM ? rsqrtf(__fmaf_rn(ss, p.inv_k, p.eps)) : 1.f;
   const float amax = __uint_as_float(mx) * o.inv;
   o.bad = !(amax < INFINITY) || (KIND == ROW_NORM && !(ss < INFINITY));
   o.amax = fmaxf(amax, AMAX_FLOOR);
@@ -238,17 +284,51 @@ VG_DEVINL void load8_raw(const char* base, long long e, int lo, int left, long l
     }
   }
 }
-// Eight 2-byte values of a group to memory: at once where the address and the row's ends allow it.
+// Group [e, e + 8) of a row of k 2-byte values, where the row may start anywhere: the 16-byte word at the next boundary takes
+// the rest from the next lane; the row's ends and the last lane's part are written one by one. All lanes call this.
+VG_DEVINL void store_half_shifted(void* row, int e, int k, uint4 own) {
+  uint16_t* dst = static_cast<uint16_t*>(row) + e;
+  const uint32_t mis = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15);           // the same in all of the row's groups
+  uint32_t t[8] = {own.x, own.y, own.z, own.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[4 + i] = __shfl_down_sync(0xffffffffu, t[i], 1);
+  if (e >= k) return;
+  const int lane = threadIdx.x & 31, head = mis ? (int)(16 - mis) / 2 : 0;          // own values before the boundary
+  const bool full = mis ? lane < 31 && e + head + 8 <= k : e + 8 <= k;
+  const bool head_done = lane > 0 && e + head <= k;                                 // by the previous lane's word
+  if (full) {
+    uint32_t s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = t[i];
+    if (head & 4) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) s[i] = s[i + 2];
+    }
+    if (head & 2) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) s[i] = s[i + 1];
+    }
+    if (head & 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = __funnelshift_r(s[i], s[i + 1], 16);
+    }
+    *reinterpret_cast<uint4*>(dst + head) = make_uint4(s[0], s[1], s[2], s[3]);
+    if (head_done) return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (!(i < head ? head_done : full) && e + i < k) dst[i] = (uint16_t)(t[i >> 1] >> (16 * (i & 1)));
+}
 template <bool VEC>
-VG_DEVINL void store8_half(void* dst, int lo, int left, uint4 v) {
-  if (VEC || (lo == 0 && left >= 8 && reinterpret_cast<uintptr_t>(dst) % 16 == 0)) {
-    *reinterpret_cast<uint4*>(dst) = v;
+VG_DEVINL void store_codes(signed char* q, int left, uint2 v) {
+  if (VEC || (left >= 8 && reinterpret_cast<uintptr_t>(q) % 8 == 0)) {
+    *reinterpret_cast<uint2*>(q) = v;
     return;
   }
   if constexpr (!VEC) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i >= lo && i < left) static_cast<uint16_t*>(dst)[i] = (uint16_t)((&v.x)[i >> 1] >> (16 * (i & 1)));
+      if (i < left) q[i] = (signed char)((&v.x)[i >> 2] >> (8 * (i & 3)));
   }
 }
 // The codes of group [e, e + 8) of a row of k, where groups start `shift` elements past multiples of eight: the 8-byte
@@ -270,17 +350,19 @@ VG_DEVINL void store_codes_shifted(signed char* q, int e, int k, int shift, uint
 
 // A row belongs to one CTA, or (CL) to a cluster of them that exchanges its partial statistics through distributed
 // shared memory. A thread owns MAXC groups of eight consecutive elements; all its loads are issued before the first use.
-// Rows that do not all start on 16-byte boundaries (!VEC) are cut into groups at the boundaries of x, so x is read and
-// written back in whole words whatever the width; the codes are shifted into their own words on the way out, with a lane's
+// Rows that do not all start on 16-byte boundaries (!VEC) are cut into groups at the boundaries of x (SHIFTED), so x is read
+// in whole words whatever the width; the codes are shifted into their own words on the way out, with a lane's
 // neighbour supplying the rest. Warps overlap by one group for that: lane 31 repeats the next warp's first. (Bytes stored
-// one by one at the seams of warps: 11.7 us at 1237 x 4111, with the overlap 8.7.)
+// one by one at the seams of warps: 11.7 us at 1237 x 4111, with the overlap 8.7.) The norm keeps the groups of aligned rows,
+// which its sum goes by, and reads and writes each from where it is.
 template <int KIND, bool VEC, int MAXC, bool CL>
 __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
   constexpr int ES = KIND == ROW_F32 ? 4 : 2;
   constexpr bool PAIR = KIND == ROW_SWIGLU || KIND == ROW_NORM;
+  constexpr bool SHIFTED = !VEC && KIND != ROW_NORM;
   __shared__ unsigned red_m[32];
-  __shared__ float red_s[32];
-  __shared__ float2 peer[MAX_CLUSTER];
+  __shared__ unsigned peer[MAX_CLUSTER];
+  __shared__ float block[KIND != ROW_NORM ? 1 : CL ? ROW_MAX / SUM_BLOCK : 32 * MAXC];
   pdl_trigger();
   if (CL) cluster_arrive_relaxed();
   pdl_wait();
@@ -292,10 +374,10 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
   const int k = p.k;
   char* x_row = static_cast<char*>(const_cast<void*>(p.x)) + row * p.ldx * ES;
   const char* d_row = reinterpret_cast<const char*>(p.delta + row * p.ldd);
-  constexpr int LANES = VEC ? 32 : 31;                             // groups of its own that a warp has
-  const int shift = VEC ? 0 : (int)((16 - (reinterpret_cast<uintptr_t>(x_row) & 15)) & 15) / ES;
+  constexpr int LANES = SHIFTED ? 31 : 32;                         // groups of its own that a warp has
+  const int shift = !SHIFTED ? 0 : (int)((16 - (reinterpret_cast<uintptr_t>(x_row) & 15)) & 15) / ES;
   const int e0 = ((tid >> 5) * LANES + (tid & 31)) * 8 - ((8 - shift) & 7), e_step = T / 32 * LANES * 8;
-  const bool owner = VEC || (tid & 31) < 31;
+  const bool owner = !SHIFTED || (tid & 31) < 31;
   uint32_t xr[MAXC][2 * ES], yr[MAXC][4];
 #pragma unroll
   for (int c = 0; c < MAXC; ++c) {
@@ -307,7 +389,7 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
     }
   }
   float v[MAXC][8];
-  float amax = 0.f, ss = 0.f;
+  float amax = 0.f, ss[MAXC] = {};
 #pragma unroll
   for (int c = 0; c < MAXC; ++c) {
     const int e = e0 + c * e_step, lo = max(0, -e);
@@ -336,7 +418,7 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
         load8_raw<VEC, 4>(reinterpret_cast<const char*>(p.w), e, lo, k - e, k, ww);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          ss += owner ? v[c][i] * v[c][i] : 0.f;
+          ss[c] = __fmaf_rn(v[c][i], v[c][i], ss[c]);
           v[c][i] *= __uint_as_float(ww[i]) + p.w_off;
         }
       }
@@ -348,20 +430,28 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
     for (int i = 0; i < 8; i += 2) amax = max_abs3(amax, v[c][i], v[c][i + 1]);
   }
   unsigned mx = __float_as_uint(amax);
-  block_reduce<KIND == ROW_NORM>(mx, ss, red_m, red_s, threadIdx.x, blockDim.x);
+  block_reduce<KIND == ROW_NORM && !CL>(mx, ss, red_m, block, threadIdx.x, blockDim.x);
   if (CL) {
+    float warps = 0.f;
+    if constexpr (KIND == ROW_NORM) warps = warp_sums(ss);
     cluster_wait();                                   // every CTA of the row has started
-    if ((int)threadIdx.x < nrank) dsmem_st_f32x2(dsmem_map(smem_u32(&peer[rank]), threadIdx.x), __uint_as_float(mx), ss);
+    if ((int)threadIdx.x < nrank) dsmem_st_u32(dsmem_map(smem_u32(&peer[rank]), threadIdx.x), mx);
+    if constexpr (KIND == ROW_NORM) {                 // each of the lanes that have a sum tells one rank
+      const int lane = tid & 31, to = lane % (32 / MAXC);
+      if (to < nrank) dsmem_st_f32(dsmem_map(smem_u32(&block[(tid >> 5) + sum_of_lane<MAXC>(lane) * (T >> 5)]), to), warps);
+    }
     cluster_sync_all();
     mx = 0;
-    ss = 0.f;
-    for (int r = 0; r < nrank; ++r) {                 // rank order: the sum does not depend on timing
-      mx = max(mx, __float_as_uint(peer[r].x));
-      ss += peer[r].y;
-    }
+    for (int r = 0; r < nrank; ++r) mx = max(mx, peer[r]);
+  }
+  float sum = 0.f;
+  if constexpr (KIND == ROW_NORM) {
+    const int blocks = (k + SUM_BLOCK - 1) / SUM_BLOCK;
+    if (CL && blocks > 128) sum = sum_of_blocks<ROW_MAX / SUM_BLOCK / 32>(block, blocks);
+    else sum = sum_of_blocks<CL ? 4 : MAXC>(block, blocks);
   }
 
-  const RowScale rs = row_scale<KIND>(p, mx, ss);
+  const RowScale rs = row_scale<KIND>(p, mx, sum);
   shrink_big_row<KIND>(v, mx);
   if (tid == 0) p.scale[row] = rs.s;
   if (KIND == ROW_NORM) {
@@ -375,12 +465,20 @@ __global__ void __launch_bounds__(1024) row_int8_kernel(const RowParams p) {
   for (int c = 0; c < MAXC; ++c) {
     const int e = e0 + c * e_step;
     const uint2 codes = rs.bad ? make_uint2(0u, 0u) : codes8<KIND>(v[c], rs);
-    if (!VEC) store_codes_shifted(p.q + row * p.ldq, e, k, shift, codes);
+    if (SHIFTED) store_codes_shifted(p.q + row * p.ldq, e, k, shift, codes);
     if (e < k && owner) {
-      if (VEC) *reinterpret_cast<uint2*>(p.q + row * p.ldq + e) = codes;
-      if (KIND == ROW_NORM && p.delta)
-        store8_half<VEC>(x_row + (long long)e * 2, max(0, -e), k - e, make_uint4(xr[c][0], xr[c][1], xr[c][2], xr[c][3]));
-      if (KIND == ROW_NORM && p.out16) store8_half<VEC>(p.out16 + row * p.ldo + e, max(0, -e), k - e, rs.bad ? nan4 : pack_f16_sat(v[c]));
+      if (!SHIFTED) store_codes<VEC>(p.q + row * p.ldq + e, k - e, codes);
+    }
+    if constexpr (KIND == ROW_NORM) {
+      const uint4 r4 = make_uint4(xr[c][0], xr[c][1], xr[c][2], xr[c][3]);
+      if (VEC && e < k) {
+        if (p.delta) *reinterpret_cast<uint4*>(x_row + (long long)e * 2) = r4;
+        if (p.out16) *reinterpret_cast<uint4*>(p.out16 + row * p.ldo + e) = rs.bad ? nan4 : pack_f16_sat(v[c]);
+      }
+      if (!VEC) {
+        if (p.delta) store_half_shifted(x_row, e, k, r4);
+        if (p.out16) store_half_shifted(p.out16 + row * p.ldo, e, k, rs.bad ? nan4 : pack_f16_sat(v[c]));
+      }
     }
   }
 }
@@ -399,7 +497,7 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ __align__(8) uint64_t full[RING_SLOTS];
   __shared__ unsigned red_m[TEAMS][2][32];
-  __shared__ float red_s[TEAMS][2][32];
+  __shared__ float block[2][KIND != ROW_NORM ? 1 : RING_GROUPS / 32];
   __shared__ int stuck[TEAMS];
   __shared__ volatile int filled[RING_SLOTS];
   constexpr int ES = KIND == ROW_F32 ? 4 : 2;
@@ -447,7 +545,7 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
     }
     const uint8_t* src = ring + (size_t)slot * slot_bytes;
     float v[MAXC][8];
-    float amax = 0.f, ss = 0.f;
+    float amax = 0.f, ss[MAXC] = {};
 #pragma unroll
     for (int c = 0; c < MAXC; ++c) {
       const int e = (tid + c * T) * 8;
@@ -478,7 +576,7 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
           const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            ss += v[c][i] * v[c][i];
+            ss[c] = __fmaf_rn(v[c][i], v[c][i], ss[c]);
             v[c][i] *= ww[i] + p.w_off;
           }
         }
@@ -490,10 +588,12 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
       for (int i = 0; i < 8; i += 2) amax = max_abs3(amax, v[c][i], v[c][i + 1]);
     }
     unsigned mx = __float_as_uint(amax);
-    block_reduce<KIND == ROW_NORM>(mx, ss, red_m[team][it & 1], red_s[team][it & 1], tid, T, team + 1);
+    block_reduce<KIND == ROW_NORM>(mx, ss, red_m[team][it & 1], block[it & 1], tid, T, team + 1);
     if (stuck[team]) break;                                // seen by the whole team: set before the barrier
     if (tid == 0 && row + (long long)slots * step < n) fill(slot, j + slots, row + (size_t)slots * step);
-    const RowScale rs = row_scale<KIND>(p, mx, ss);
+    float sum = 0.f;
+    if constexpr (KIND == ROW_NORM) sum = sum_of_blocks<MAXC == 4 ? (RING_GROUPS / 32 + 31) / 32 : 1>(block[it & 1], (k + SUM_BLOCK - 1) / SUM_BLOCK);
+    const RowScale rs = row_scale<KIND>(p, mx, sum);
     shrink_big_row<KIND>(v, mx);
     if (tid == 0) p.scale[row] = rs.s;
 #pragma unroll
@@ -599,15 +699,14 @@ constexpr int RING_PER_SM = 16;                   // blocks per SM
 constexpr int RING_MIN_ROWS = 8;                  // rows per SM from which the ring form pays
 constexpr int RING_MIN_WIDE = 1;                  // the same for rows of more than 8192
 
-// Largest row width: a cluster of eight CTAs of 1024 threads with two (three) groups of eight each.
-constexpr int ROW_MAX = MAX_CLUSTER * 1024 * 2 * 8;
-
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 template <int KIND, bool VEC>
 cudaError_t launch_shape(RowParams p, int n, cudaStream_t st) {
-  // without VEC a row may begin and end inside a group, and a warp has 31 of its own
-  const int groups = VEC ? p.k / 8 : (p.k + 14) / 8, lanes = VEC ? 32 : 31;
+  // shifted rows may begin and end inside a group, and a warp has 31 of its own
+  constexpr bool SHIFTED = !VEC && KIND != ROW_NORM;
+  const int groups = SHIFTED ? (p.k + 14) / 8 : (p.k + 7) / 8;
+  constexpr int lanes = SHIFTED ? 31 : 32;
   auto threads = [&](int parts) { return dim3((groups + parts * lanes - 1) / (parts * lanes) * 32); };
   p.cluster = 1;
   // many shifted rows without a second input: two groups a thread halve the fixed instructions (4096 x 4111 quantise: 25.3
@@ -616,9 +715,11 @@ cudaError_t launch_shape(RowParams p, int n, cudaStream_t st) {
   if (groups <= 32 * lanes && !two) return launch_pdl(row_int8_kernel<KIND, VEC, 1, false>, dim3(n), threads(1), 0, st, p);
   if (groups <= 64 * lanes) return launch_pdl(row_int8_kernel<KIND, VEC, 2, false>, dim3(n), threads(2), 0, st, p);
   while (p.cluster < MAX_CLUSTER && p.cluster * 64 * lanes < groups) p.cluster *= 2;
-  if (VEC || groups <= p.cluster * 64 * lanes)
-    return launch_pdl_cluster(row_int8_kernel<KIND, VEC, 2, true>, dim3(n * p.cluster), threads(2 * p.cluster), p.cluster, 0, st, p);
-  return launch_pdl_cluster(row_int8_kernel<KIND, false, 3, true>, dim3(n * p.cluster), threads(3 * p.cluster), p.cluster, 0, st, p);
+  if constexpr (SHIFTED) {
+    if (groups > p.cluster * 64 * lanes)
+      return launch_pdl_cluster(row_int8_kernel<KIND, false, 3, true>, dim3(n * p.cluster), threads(3 * p.cluster), p.cluster, 0, st, p);
+  }
+  return launch_pdl_cluster(row_int8_kernel<KIND, VEC, 2, true>, dim3(n * p.cluster), threads(2 * p.cluster), p.cluster, 0, st, p);
 }
 
 int sm_count() {
@@ -663,7 +764,7 @@ int launch_row(const RowParams& p, int n, int esize, cudaStream_t st) {
     if (p.out16) vec = vec && aligned(p.out16, 16) && (n == 1 || p.ldo % 8 == 0);
   }
   const int sms = sm_count(), slot = p.k * esize * ((KIND == ROW_SWIGLU || p.delta) ? 2 : 1), groups = p.k / 8;
-  if (vec && n >= (groups > 1024 ? RING_MIN_WIDE : RING_MIN_ROWS) * sms && slot % 16 == 0 && 2 * slot <= RING_BYTES && groups <= 2560) {
+  if (vec && n >= (groups > 1024 ? RING_MIN_WIDE : RING_MIN_ROWS) * sms && slot % 16 == 0 && 2 * slot <= RING_BYTES && groups <= RING_GROUPS) {
     if constexpr (KIND == ROW_SWIGLU) {
       if (4 * slot > RING_BYTES && groups > 1024) return launch_ring<KIND, 5, 2>(p, n, slot, sms, st);
     }
@@ -713,7 +814,7 @@ extern "C" int vg_add_rmsnorm_int8(void* res, long long ld_res, const void* delt
                                    long long ld_out16, int* err, cudaStream_t st) {
   RowParams p{};
   p.x = res; p.ldx = ld_res; p.delta = static_cast<const __nv_bfloat16*>(delta); p.ldd = ld_delta; p.w = w; p.k = h;
-  p.eps = eps; p.w_off = plus_one ? 1.0f : 0.0f; p.q = static_cast<signed char*>(q); p.ldq = ldq; p.scale = scale; p.err = err;
+  p.eps = eps; p.inv_k = h > 0 ? 1.0f / (float)h : 0.f; p.w_off = plus_one ? 1.0f : 0.0f; p.q = static_cast<signed char*>(q); p.ldq = ldq; p.scale = scale; p.err = err;
   p.out16 = static_cast<__half*>(out16); p.ldo = ld_out16;
   return launch_row<ROW_NORM>(p, n, 2, st);
 }

@@ -547,3 +547,38 @@ def test_every_pair_of_16_bit_significands(dtype, bits, exps):
         act = I8.quantize_act_int8(x)
         codes, scale = _exact_codes(x)
         assert torch.equal(act.scale, scale) and torch.equal(act.q, codes), exp
+
+
+# ring form (one, two, four groups a thread) against the row form alone and in clusters; odd widths; every start within 16 bytes
+@pytest.mark.parametrize("n,k", [(1300, 256), (1300, 2048), (1200, 5120), (150, 8200), (170, 17408), (149, 20480), (7, 40000),
+                                 (1200, 2051), (300, 8209), (5, 131071)])
+def test_norm_of_a_row_does_not_depend_on_the_call(n, k):
+    """A row's codes, scale and f16 copy have the same bits alone, among a few and among many, with and without a residual
+    update, aligned or not."""
+    from velogb10_b200.ops import int8 as I8
+    res, w = _randn((n, k), k, BF) * 3, _randn((k,), n) * 0.3
+    many, f16 = res.clone(), torch.empty((n, k), dtype=F16, device="cuda")
+    act = I8.add_rmsnorm_int8(many, None, w, 1e-6, out16=f16)
+    rows = sorted({0, 1, 2, 3, n // 2, n - 2, n - 1})
+    for lo, hi in [(r, r + 1) for r in rows] + [(0, min(n, 5)), (n // 3, min(n, n // 3 + 100))]:
+        for off in (0, 1, 3, 4):
+            x = torch.zeros((hi - lo, k + 8), dtype=BF, device="cuda")[:, off:off + k]
+            x.copy_(res[lo:hi])
+            d, o = (torch.zeros_like(x), torch.empty((hi - lo, k), dtype=F16, device="cuda"))
+            got = I8.add_rmsnorm_int8(x, d if off else None, w, 1e-6, out16=o)
+            assert torch.equal(got.q, act.q[lo:hi]) and torch.equal(got.scale, act.scale[lo:hi]) and torch.equal(o, f16[lo:hi]), (lo, hi, off)
+    _check_rows(act, res.double() * torch.rsqrt(res.double().square().mean(-1, keepdim=True) + 1e-6) * (1 + w.double()), n,
+                27 * 2.0 ** -24, (n, k))
+
+
+@pytest.mark.parametrize("n,k", [(1300, 512), (1200, 5120), (150, 8200), (333, 17408), (149, 20480)])
+def test_swiglu_of_a_row_does_not_depend_on_the_call(n, k):
+    from velogb10_b200.ops import int8 as I8
+    gu = _randn((n, 2 * k), k, BF) * 2
+    act = I8.swiglu_int8(gu)
+    for lo, hi in ((0, 1), (n - 1, n), (n // 2, n // 2 + 40)):
+        for off in (0, 1):
+            x = torch.zeros((hi - lo, 2 * k + 8), dtype=BF, device="cuda")[:, off:off + 2 * k]
+            x.copy_(gu[lo:hi])
+            got = I8.swiglu_int8(x)
+            assert torch.equal(got.q, act.q[lo:hi]) and torch.equal(got.scale, act.scale[lo:hi]), (lo, hi, off)

@@ -7,6 +7,9 @@ too, once, at load (``codec.quantize_int8``, ``QLinear.from_dense(w, "int8")``).
 ``out[i, m] = (sum_k q[i, k] c[m, k]) * s[i] * row_scale[m]`` has an exact integer sum, so it depends neither on the batch
 width nor on how the kernel splits K.
 
+No result of a token depends on the other rows of the call, on their number or on where its row lies: the norm sums a row's
+squares in one order that goes by the width alone.
+
 A row that holds an infinity or a NaN gets scale NaN and codes 0: all that is computed from it is NaN.
 
 Wrappers check their arguments before anything is enqueued (``KernelError``), launch on the current stream of the
