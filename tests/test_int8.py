@@ -188,3 +188,23 @@ def test_codec_rounds_exact_halves_to_even():
     assert half.sum() > 20
     assert torch.equal(q.codes.long(), want)
     assert torch.equal(q.row_scale, (amax.squeeze(-1).double() * 2.0 ** -20 / 127).float())
+
+
+def test_norm_behind_a_pending_reduction_quantises_the_residual(monkeypatch):
+    """Tensor-parallel decode widths leave a sum to the norm kernel, longer inputs do not. The int8 rows come from the fp32 norm
+    of the residual in both cases, not from the f16 copy."""
+    from types import SimpleNamespace
+    from velogb10_b200.models import runtime
+    calls = []
+    monkeypatch.setattr(runtime.G, "add_rmsnorm_fp4_ar", lambda *a, **k: calls.append("sum") or ("bq", "sfb", "g0"))
+    monkeypatch.setattr(runtime.I8, "add_rmsnorm_int8", lambda res, delta, w, eps, n, **k: calls.append((res, delta, n, k["out"])) or k["out"])
+    gm = object.__new__(runtime.GpuModel)
+    gm.cfg, gm.comm, gm.use_fp4 = SimpleNamespace(rms_eps=1e-6), None, True
+    x, out = torch.zeros(16, 32, dtype=BF), _act(16, 32)
+    ws = SimpleNamespace(x=x, xn16=torch.zeros(16, 32, dtype=F16), delta=torch.zeros_like(x), i8=lambda width, tag="": out)
+    for mode in (1, 2):
+        gm._pending_ar, calls[:] = mode, []
+        assert gm._norm(ws, ws.delta, torch.zeros(32), 3, _w(8, 32)) is out
+        assert calls[0] == "sum" and calls[1][0] is x and calls[1][1] is None and calls[1][2] == 3 and gm._pending_ar == 0
+    gm._pending_ar = 1
+    assert gm._norm(ws, ws.delta, torch.zeros(32), 3, QLinear("nvfp4", 16, 32)) == ("bq", "sfb", "g0")

@@ -401,10 +401,14 @@ class GpuModel:
         activation series, returned for the linears that read this input. When the preceding row-parallel
         linear only pushed its partial rows (``self._pending_ar``), the kernel also performs the
         tensor-parallel sum. When the linear ``q`` that reads the result has int8 weights, the same kernel emits
-        int8 rows instead."""
+        int8 rows instead; behind a pending sum a second launch makes them from the residual, in fp32 as at any width
+        (from ``ws.xn16``, which is rounded, a row's codes would depend on the width)."""
         if self._pending_ar:
             mode, self._pending_ar = self._pending_ar, 0
-            return G.add_rmsnorm_fp4_ar(ws.x, w, self.cfg.rms_eps, n, self.comm, out16=ws.xn16, mode=mode)
+            act = G.add_rmsnorm_fp4_ar(ws.x, w, self.cfg.rms_eps, n, self.comm, out16=ws.xn16, mode=mode)
+            if q is not None and q.fmt == "int8":
+                return I8.add_rmsnorm_int8(ws.x, None, w, self.cfg.rms_eps, n, out=ws.i8(ws.x.shape[1]))
+            return act
         if q is not None and q.fmt == "int8":
             return I8.add_rmsnorm_int8(ws.x, delta, w, self.cfg.rms_eps, n, out=ws.i8(ws.x.shape[1]), out16=ws.xn16)
         if self.use_fp4 and n <= 16 and ws.x.shape[1] % 16 == 0:
