@@ -300,6 +300,7 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
       }
     }
   } else if (warp == 1) {
+    pdl_wait();                                           // no stage fills before: the bounded waits time this kernel's work only
     constexpr uint32_t idesc = idesc_i8(BM, BN);
     const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), bdesc0 = umma_desc_sw128(smem_u32(smem) + A_BYTES);
     int st = 0;
@@ -511,6 +512,7 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
     // slab a stage: 296 cycles a slab at any BN up to 128. With a warp index the compiler cannot know to be uniform, 388.
     // With the loop inside a lane == 0 branch, 330 and 70 for each MMA.)
     if (rank == 0) {
+      pdl_wait();                                                    // as above
       const uint32_t idesc = idesc_i8(2 * BM, sh.bn);
       const uint16_t mask = (uint16_t)(3u << leader);
       const uint64_t adesc0 = umma_desc_sw128(smem_u32(smem)), bdesc0 = umma_desc_sw128(smem_u32(smem) + sh.per * A_BYTES);
