@@ -178,6 +178,9 @@ VG_DEVINL float dsmem_ld_f32(uint32_t addr) {
   return v;
 }
 
+VG_DEVINL void dsmem_st_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 VG_DEVINL void dsmem_st_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }

@@ -186,15 +186,13 @@ VG_DEVINL void fetch_sx(const I8Params& p, float* sx, int n0, int cols) {
 VG_DEVINL uint32_t group_slots(int cols, int parts) { return (uint32_t)(((cols + 3) / 4 + parts - 1) / parts); }
 // `to_rank(part)`: cluster rank of the CTA of that part which holds the same channels
 template <typename F>
-VG_DEVINL void send_partials(uint32_t area, uint32_t acc, bool have, int cols, int part, int parts, int r, int turn, int of, F to_rank) {
+VG_DEVINL void send_partials(uint32_t area, uint32_t acc, int cols, int part, int parts, int r, int turn, int of, F to_rank) {
   const uint32_t slots = group_slots(cols, parts);
   for (int c = turn * 16; c < cols; c += of * 16) {
     uint32_t v[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    if (have) {
-      tmem_ld8(acc + c, v);
-      if (c + 8 < cols) tmem_ld8(acc + c + 8, v + 8);
-      tmem_ld_wait();
-    }
+    tmem_ld8(acc + c, v);
+    if (c + 8 < cols) tmem_ld8(acc + c + 8, v + 8);
+    tmem_ld_wait();
     uint32_t slot = (uint32_t)(c / 4) / (uint32_t)parts;
     int dst = c / 4 - (int)slot * parts;
 #pragma unroll
@@ -203,6 +201,12 @@ VG_DEVINL void send_partials(uint32_t area, uint32_t acc, bool have, int cols, i
       if (++dst == parts) { dst = 0; ++slot; }
     }
   }
+}
+// A part whose accumulator never came tells every part, itself among them: none stores a sum that lacks a piece of K.
+template <typename F>
+VG_DEVINL void report_lost(const volatile int* lost, int parts, F to_rank) {
+  const int lane = threadIdx.x & 31;
+  if (lane < parts) dsmem_st_u32(dsmem_map(smem_u32(const_cast<const int*>(lost)), to_rank(lane)), 1u);
 }
 template <int G>
 VG_DEVINL void finish_partials(const I8Params& p, const uint8_t* area, const OutWarp& o, const float* sx, int cols, int part, int parts,
@@ -253,6 +257,7 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   uint64_t* acc_full = empty + S::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* lost = abort_flag + 1;                   // split: some part of this tile has no sums to send
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? uniform((int)cluster_ctarank()) : 0;
@@ -273,6 +278,7 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
     }
     mbar_init(acc_full, 1);
     *abort_flag = 0;
+    *lost = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -342,15 +348,19 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
     }
   } else {
     cluster_sync_all();                                    // every CTA's MMAs are done: the rings are free
-    if (warp >= 2) send_partials(smem_u32(smem), lane_base, have, cols, rank, p.split, r, 0, 1, [](int q) { return (uint32_t)q; });
+    auto to_rank = [](int q) { return (uint32_t)q; };
+    if (warp >= 2) {
+      if (have) send_partials(smem_u32(smem), lane_base, cols, rank, p.split, r, 0, 1, to_rank);
+      else report_lost(lost, p.split, to_rank);
+    }
     cluster_sync_all();
-    if (warp >= 2) finish_partials<2>(p, smem, OutWarp(p, m0 + r, n0), sx, cols, rank, p.split, r, 0, 1);
-  }
-  if (*abort_flag && threadIdx.x == 0) {
-    for (int i = 0; i < 64; ++i) __nanosleep(1000);       // let copies in flight land before the block ends
+    if (warp >= 2 && !*lost) finish_partials<2>(p, smem, OutWarp(p, m0 + r, n0), sx, cols, rank, p.split, r, 0, 1);
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);       // let copies and MMAs in flight end before the block does
+  }
   if (warp == 1) tmem_dealloc(tmem, S::TMEM_COLS);
 }
 
@@ -426,6 +436,7 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   uint64_t* acc_empty = acc_full + 2;                                // [2], the leader's counts both CTAs' epilogue warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* lost = abort_flag + 1;                   // split: some part of this tile has no sums to send
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int crank = uniform((int)cluster_ctarank());
@@ -455,6 +466,7 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
       mbar_init(acc_empty + i, 2 * P_EPI);
     }
     *abort_flag = 0;
+    *lost = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -466,7 +478,12 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   cluster_sync_all();                                                // both CTAs' barriers are set up
   tc_fence_after();
   const uint32_t tmem = uniform(*tmem_slot);
-  auto fail = [&](int code) { if (p.err) atomicCAS(p.err, 0, code); *abort_flag = 1; };
+  // both CTAs of the pair have to know: copies of either signal the leader, MMAs read both
+  auto fail = [&](int code) {
+    if (p.err) atomicCAS(p.err, 0, code);
+    *abort_flag = 1;
+    dsmem_st_u32(dsmem_map(smem_u32(const_cast<const int*>(abort_flag)), crank ^ 1), 1u);
+  };
 
   const int quarter = warp & 3;
   const int r = quarter * 32 + lane;                                 // channel of this thread within the CTA's 128
@@ -572,18 +589,20 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
     sh.tiles.at(first, mi, ni);
     const int n0 = ni * sh.bn, cols = min(sh.bn, p.N - n0);
     cluster_sync_all();                                              // every CTA's MMAs are done: the rings are free
-    if (warp >= 2)
-      send_partials(smem_u32(smem), tmem + ((uint32_t)(quarter * 32) << 16), have, cols, part, p.split, r, turn, 2,
-                    [rank](int q) { return (uint32_t)(2 * q + rank); });
+    auto to_rank = [rank](int q) { return (uint32_t)(2 * q + rank); };
+    if (warp >= 2) {
+      if (have) send_partials(smem_u32(smem), tmem + ((uint32_t)(quarter * 32) << 16), cols, part, p.split, r, turn, 2, to_rank);
+      else report_lost(lost, p.split, to_rank);
+    }
     cluster_sync_all();
-    if (warp >= 2) finish_partials<2>(p, smem, OutWarp(p, mi * 2 * BM + rank * BM + r, n0), sx, cols, part, p.split, r, turn, 2);
-  }
-  if (*abort_flag && threadIdx.x == 0) {
-    for (int i = 0; i < 64; ++i) __nanosleep(1000);       // let copies in flight land before the block ends
+    if (warp >= 2 && !*lost) finish_partials<2>(p, smem, OutWarp(p, mi * 2 * BM + rank * BM + r, n0), sx, cols, part, p.split, r, turn, 2);
   }
   tc_fence_before();
   __syncwarp();
   cluster_sync_all();
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);       // let copies and MMAs in flight end before the blocks do
+  }
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 

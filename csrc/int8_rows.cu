@@ -57,9 +57,6 @@ VG_DEVINL float max_abs3(float m, float a, float b) {
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
   return r;
 }
-VG_DEVINL void dsmem_st_u32(uint32_t addr, unsigned v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
 
 // The sum of a norm row's squares has one order whatever form runs the row, where it lies and how many rows there are, so a
 // token's codes do not depend on the batch: groups of eight consecutive elements one after the other, blocks of 32 groups
