@@ -264,7 +264,6 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   const int m0 = (blockIdx.x / p.split) * BM, n0 = blockIdx.y * BN;
   const int slabs = (p.K + BK - 1) / BK;
   const int s0 = (int)((long long)slabs * rank / p.split), s1 = (int)((long long)slabs * (rank + 1) / p.split);
-  pdl_trigger();
 
   if (warp == 0 && elect_one()) {
     tma_prefetch_desc(&tm_w);
@@ -288,6 +287,8 @@ gemm_int8_kernel(const I8Params p, const __grid_constant__ CUtensorMap tm_w, con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Not before the allocation: a dependent that takes all 512 columns first would wait for this grid, and this grid for it.
+  pdl_trigger();
   const uint32_t tmem = uniform(*tmem_slot);
   auto fail = [&](int code) { if (p.err) atomicCAS(p.err, 0, code); *abort_flag = 1; };
 
@@ -447,7 +448,6 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   const int slabs = (p.K + BK - 1) / BK;
   const int s0 = SPLIT ? (int)((long long)slabs * part / p.split) : 0;
   const int s1 = SPLIT ? (int)((long long)slabs * (part + 1) / p.split) : slabs;
-  pdl_trigger();
 
   if (warp == 0 && elect_one()) {
     tma_prefetch_desc(&tm_w);
@@ -477,6 +477,7 @@ gemm_int8_pair_kernel(const I8Params p, const PairShape sh, const __grid_constan
   __syncthreads();
   cluster_sync_all();                                                // both CTAs' barriers are set up
   tc_fence_after();
+  pdl_trigger();                                                     // not before the allocation, as above
   const uint32_t tmem = uniform(*tmem_slot);
   // both CTAs of the pair have to know: copies of either signal the leader, MMAs read both
   auto fail = [&](int code) {

@@ -50,3 +50,11 @@ def test_failed_blocks_outlive_their_copies():
         assert body.rindex("fail(VG_ERR") < body.rindex(last) < look < body.index("dealloc"), name
         assert "__nanosleep" in body[look:]
     assert "smem_u32(const_cast<const int*>(abort_flag)), crank ^ 1)" in _body("gemm_int8_pair_kernel")
+
+
+def test_dependents_start_behind_the_tensor_memory_allocation():
+    """A dependent kernel may allocate all of an SM's tensor memory and then wait for this grid to end. Were this grid's own
+    allocation still to come, neither would move on."""
+    for name, alloc in (("gemm_int8_kernel", "tmem_alloc("), ("gemm_int8_pair_kernel", "tcgen05.alloc")):
+        body = _body(name)
+        assert body.index(alloc) < body.index("__syncthreads()") < body.index("pdl_trigger()"), name
