@@ -208,3 +208,34 @@ def test_norm_behind_a_pending_reduction_quantises_the_residual(monkeypatch):
         assert calls[0] == "sum" and calls[1][0] is x and calls[1][1] is None and calls[1][2] == 3 and gm._pending_ar == 0
     gm._pending_ar = 1
     assert gm._norm(ws, ws.delta, torch.zeros(32), 3, QLinear("nvfp4", 16, 32)) == ("bq", "sfb", "g0")
+
+
+def _builder(tensors):
+    from velogb10_b200.config import tiny_hybrid
+    from velogb10_b200.models.weights import DictSource, ModelBuilder
+    return ModelBuilder(tiny_hybrid(False), DictSource(tensors))
+
+
+def test_checkpoint_scales_and_zero_points():
+    """What stands beside int8 codes decides what they mean: other layouts than a scale a row are refused at load."""
+    g = torch.Generator().manual_seed(0)
+    a = codec.quantize_int8(torch.randn(32, 48, generator=g))
+    name = "layers.0.mlp.up_proj"
+    base = {name + ".weight": a.codes, name + ".weight_scale": a.row_scale[:, None]}
+    zeros = torch.zeros(32, 1, dtype=torch.int8)
+    q = _builder({**base, name + ".weight_zero_point": zeros}).linear(name)
+    assert torch.equal(q.codes, a.codes) and torch.equal(q.row_scale, a.row_scale)
+    one = _builder({**base, name + ".weight_scale": torch.tensor([0.5]).bfloat16()}).linear(name)
+    assert one.row_scale.shape == (32,) and one.row_scale.is_contiguous() and (one.row_scale == 0.5).all()
+    assert torch.equal(one.dequant(), a.codes.float() * 0.5)
+    for extra, what in (({name + ".weight_zero_point": zeros + 1}, "zero point"),
+                        ({name + ".weight_scale": torch.ones(32, 3)}, "96 scales for 32"),
+                        ({name + ".weight_scale": torch.ones(31)}, "31 scales for 32")):
+        with pytest.raises(ValueError, match=what):
+            _builder({**base, **extra}).linear(name)
+    with pytest.raises(ValueError, match="without a weight_scale"):
+        _builder({name + ".weight": a.codes}).linear(name)
+    head = {"lm_head.weight": a.codes, "lm_head.weight_scale": a.row_scale}          # decoded to bf16: the same rules
+    with pytest.raises(ValueError, match="zero point"):
+        _builder({**head, "lm_head.weight_zero_point": zeros + 1}).linear("lm_head")
+    assert torch.equal(_builder({**head, "lm_head.weight_scale": torch.tensor(2.0)}).linear("lm_head").w, (a.codes.float() * 2).bfloat16())
