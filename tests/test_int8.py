@@ -239,3 +239,24 @@ def test_checkpoint_scales_and_zero_points():
     with pytest.raises(ValueError, match="zero point"):
         _builder({**head, "lm_head.weight_zero_point": zeros + 1}).linear("lm_head")
     assert torch.equal(_builder({**head, "lm_head.weight_scale": torch.tensor(2.0)}).linear("lm_head").w, (a.codes.float() * 2).bfloat16())
+
+
+def test_requant_re_encodes_int8_gdn_projections(tmp_path):
+    """``gdn4`` means GDN projections in NVFP4, whatever 8-bit format they came in; the int8 MLP stays as it is."""
+    from velogb10_b200.checkpoint import io
+    from velogb10_b200.checkpoint.synthetic import synthetic_state_dict
+    from velogb10_b200.config import tiny_hybrid
+    from velogb10_b200.models.weights import ModelBuilder
+    cfg = tiny_hybrid(False)
+    a, b = str(tmp_path / "a"), str(tmp_path / "b")
+    io.write_checkpoint(a, synthetic_state_dict(cfg, seed=0).items(), cfg.to_hf_dict(), "all,mlp:int8,gdn:int8")
+    stats = io.requant_gdn(a, b)
+    before = dict(ModelBuilder(cfg, io.SafetensorsSource(a)).build().linears())
+    after = dict(ModelBuilder(cfg, io.SafetensorsSource(b)).build().linears())
+    gdn = [n for n in before if n.endswith(("in_proj", "gdn.out")) or ".gdn" in n]
+    assert stats["requant"] > 0 and gdn and all(before[n].fmt == "int8" and after[n].fmt == "nvfp4" for n in gdn)
+    for n in before:
+        if n not in gdn:
+            assert before[n].fmt == after[n].fmt
+            if before[n].fmt == "int8":
+                assert torch.equal(before[n].codes, after[n].codes) and torch.equal(before[n].row_scale, after[n].row_scale)

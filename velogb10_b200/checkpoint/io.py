@@ -407,7 +407,7 @@ def quantize_checkpoint(in_dir: str, out_dir: str, recipe: str = "all,gdn:fp8",
 
 
 def requant_gdn(from_dir: str, out_dir: str, max_shard_bytes: int = 12 << 30) -> dict:
-    """Derive a ``gdn4`` checkpoint from a mixed one: FP8 GDN in/out projections are decoded to bf16
+    """Derive a ``gdn4`` checkpoint from a mixed one: FP8 (and int8) GDN in/out projections are decoded to bf16
     and re-encoded as NVFP4; every other tensor is copied verbatim (reference: src/main.rs:1897-1999)."""
     src = SafetensorsSource(from_dir)
     with open(os.path.join(from_dir, "config.json")) as f:
@@ -420,10 +420,13 @@ def requant_gdn(from_dir: str, out_dir: str, max_shard_bytes: int = 12 << 30) ->
         t = None
         if ".linear_attn." in n and n.endswith(".weight") and ("in_proj" in n or "out_proj" in n):
             t = src.get(n)
-            if t.dtype == torch.float8_e4m3fn and t.dim() == 2 and t.shape[0] % 16 == 0 and t.shape[1] % 16 == 0:
+            if t.dtype in (torch.float8_e4m3fn, torch.int8) and t.dim() == 2 and t.shape[0] % 16 == 0 and t.shape[1] % 16 == 0:
                 stem = n[:-len(".weight")]
-                rs = src.get(stem + ".weight_scale").float()
-                bf = codec.dequantize_fp8(t.view(torch.uint8), rs)
+                if t.dtype == torch.int8:
+                    bf = codec.dequantize_int8(t, codec.int8_row_scales(stem, t, src.get))
+                    skip.add(stem + ".weight_zero_point")
+                else:
+                    bf = codec.dequantize_fp8(t.view(torch.uint8), src.get(stem + ".weight_scale").float())
                 q = codec.quantize_nvfp4(bf)
                 w.add(stem + ".weight_packed", q.packed)
                 w.add(stem + ".weight_scale", q.scales.view(torch.float8_e4m3fn))

@@ -359,7 +359,7 @@ class ModelBuilder:
             return self._maybe_dequant(QLinear("fp8", c.shape[0], c.shape[1], codes=c.contiguous(), row_scale=rs,
                                                experts=experts))
         if w.dtype == torch.int8:
-            rs = self._int8_scales(stem, w).to(self.device)
+            rs = codec.int8_row_scales(stem, w, self._t).to(self.device)
             if w.dim() == 3 or group_of(stem + suffix) not in INT8_GROUPS:       # no int8 kernels for these: bf16
                 dense = w.to(self.device).float() * rs.reshape(w.shape[:-1]).unsqueeze(-1)
                 return QLinear.from_dense(dense.to(torch.bfloat16), "bf16")
@@ -376,21 +376,6 @@ class ModelBuilder:
                 self.fake_quant_stats.append((stem + suffix, fq, err))
                 return QLinear.from_dense(back.to(torch.bfloat16), "bf16")
         return QLinear.from_dense(w, fmt)
-
-    def _int8_scales(self, stem: str, w: torch.Tensor) -> torch.Tensor:
-        """fp32 scale of every row of an int8 checkpoint tensor. Symmetric codes with one scale a row, or one for the whole
-        tensor, are what the codes mean here; anything else beside them would be a different matrix."""
-        rs = self._t(stem + ".weight_scale")
-        if rs is None:
-            raise ValueError(f"{stem}: int8 weights without a weight_scale")
-        zero = self._t(stem + ".weight_zero_point")
-        if zero is not None and bool((zero != 0).any()):
-            raise ValueError(f"{stem}: int8 weights with a zero point (asymmetric codes) are not supported")
-        rows = w.numel() // w.shape[-1]
-        if rs.numel() not in (1, rows):
-            raise ValueError(f"{stem}: {rs.numel()} scales for {rows} int8 rows (one a row or one in all is supported, groups "
-                             f"within a row are not)")
-        return rs.float().reshape(-1).expand(rows).contiguous()
 
     def _maybe_dequant(self, q: QLinear) -> QLinear:
         if not self.dequant_at_load:

@@ -206,6 +206,23 @@ def dequantize_int8(codes: torch.Tensor, row_scale: torch.Tensor, dtype=torch.bf
     return (codes.float() * row_scale.float().unsqueeze(-1)).to(dtype)
 
 
+def int8_row_scales(stem: str, w: torch.Tensor, get) -> torch.Tensor:
+    """fp32 scale of every row of the int8 checkpoint tensor ``w`` named ``stem``; ``get(name)`` returns what is stored beside
+    it, or None. Symmetric codes with one scale a row, or one for the whole tensor, are what the codes mean here; anything else
+    beside them would be a different matrix."""
+    rs = get(stem + ".weight_scale")
+    if rs is None:
+        raise ValueError(f"{stem}: int8 weights without a weight_scale")
+    zero = get(stem + ".weight_zero_point")
+    if zero is not None and bool((zero != 0).any()):
+        raise ValueError(f"{stem}: int8 weights with a zero point (asymmetric codes) are not supported")
+    rows = w.numel() // w.shape[-1]
+    if rs.numel() not in (1, rows):
+        raise ValueError(f"{stem}: {rs.numel()} scales for {rows} int8 rows (one a row or one in all is supported, groups "
+                         f"within a row are not)")
+    return rs.float().reshape(-1).expand(rows).contiguous()
+
+
 # ------------------------------------------------------------------ helpers
 
 def fake_quant(w: torch.Tensor, fmt: str) -> torch.Tensor:
