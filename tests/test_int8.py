@@ -260,3 +260,25 @@ def test_requant_re_encodes_int8_gdn_projections(tmp_path):
             assert before[n].fmt == after[n].fmt
             if before[n].fmt == "int8":
                 assert torch.equal(before[n].codes, after[n].codes) and torch.equal(before[n].row_scale, after[n].row_scale)
+
+
+def test_checkpoint_names_its_layout(tmp_path):
+    import json
+    from velogb10_b200.checkpoint import io
+    from velogb10_b200.checkpoint.synthetic import synthetic_state_dict
+    from velogb10_b200.config import tiny_hybrid
+    cfg = tiny_hybrid(False)
+
+    def label(d):
+        return json.load(open(d + "/config.json"))["quantization_config"]["format"]
+
+    for i, (recipe, want, after) in enumerate((("all", "nvfp4-pack-quantized", "nvfp4-pack-quantized"),
+                                               ("all,gdn:fp8", "nvfp4-pack-quantized", "nvfp4-pack-quantized"),
+                                               ("all,gdn:int8", "mixed-precision", "nvfp4-pack-quantized"),
+                                               ("all,mlp:int8,gdn:int8", "mixed-precision", "mixed-precision"),
+                                               ("mlp:int8,attn:int8,gdn:int8", "int-quantized", "mixed-precision"))):
+        a, b = str(tmp_path / f"a{i}"), str(tmp_path / f"b{i}")
+        io.write_checkpoint(a, synthetic_state_dict(cfg, seed=0).items(), cfg.to_hf_dict(), recipe)
+        assert label(a) == want
+        io.requant_gdn(a, b)
+        assert label(b) == after

@@ -369,6 +369,14 @@ def _iter_fused(named: Iterable[Tuple[str, torch.Tensor]], n_experts: Optional[i
         yield from _fuse_expert_set(base, d, n)
 
 
+def _format_label(n_int8: int, n_other: int) -> str:
+    """compressed-tensors' name of a layout: its readers take the linears of a checkpoint that is not "mixed-precision" for
+    tensors of the one format."""
+    if n_int8 == 0:
+        return "nvfp4-pack-quantized"
+    return "mixed-precision" if n_other else "int-quantized"
+
+
 def write_checkpoint(out_dir: str, named: Iterable[Tuple[str, torch.Tensor]], config: dict,
                      recipe: str = "all,gdn:fp8", max_shard_bytes: int = 12 << 30,
                      sidecar_dir: Optional[str] = None) -> dict:
@@ -384,7 +392,7 @@ def write_checkpoint(out_dir: str, named: Iterable[Tuple[str, torch.Tensor]], co
     cfg = dict(config)
     if rec is not None:
         cfg["quantization_config"] = {"quant_method": "compressed-tensors",
-                                      "format": "nvfp4-pack-quantized", "recipe": recipe}
+                                      "format": _format_label(stats.get("int8", 0), stats["nvfp4"] + stats["fp8"]), "recipe": recipe}
     with open(os.path.join(out_dir, "config.json"), "w") as f:
         json.dump(cfg, f, indent=1)
     if sidecar_dir:
@@ -416,6 +424,7 @@ def requant_gdn(from_dir: str, out_dir: str, max_shard_bytes: int = 12 << 30) ->
     stats = {"requant": 0, "copied": 0}
     names = src.names()
     skip = set()
+    int8_left = 0
     for n in names:
         t = None
         if ".linear_attn." in n and n.endswith(".weight") and ("in_proj" in n or "out_proj" in n):
@@ -437,11 +446,15 @@ def requant_gdn(from_dir: str, out_dir: str, max_shard_bytes: int = 12 << 30) ->
     for n in names:
         if n in skip:
             continue
-        w.add(n, src.get(n))
+        t = src.get(n)
+        int8_left += t.dtype == torch.int8 and not n.endswith(".weight_zero_point")
+        w.add(n, t)
         stats["copied"] += 1
     w.finish()
-    config.setdefault("quantization_config", {"quant_method": "compressed-tensors",
-                                              "format": "nvfp4-pack-quantized"})["recipe"] = "gdn4"
+    quant = config.setdefault("quantization_config", {"quant_method": "compressed-tensors"})
+    quant["recipe"] = "gdn4"
+    if "format" not in quant or quant["format"] in ("mixed-precision", "int-quantized"):
+        quant["format"] = _format_label(int8_left, 1)
     with open(os.path.join(out_dir, "config.json"), "w") as f:
         json.dump(config, f, indent=1)
     for sn in SIDECARS:
