@@ -582,3 +582,19 @@ def test_swiglu_of_a_row_does_not_depend_on_the_call(n, k):
             x.copy_(gu[lo:hi])
             got = I8.swiglu_int8(x)
             assert torch.equal(got.q, act.q[lo:hi]) and torch.equal(got.scale, act.scale[lo:hi]), (lo, hi, off)
+
+
+def test_without_pytorchs_private_calls(monkeypatch):
+    from velogb10_b200.ops import int8 as I8, lib
+    x, q = _randn((5, 300), 1, BF), _weights(64, 300, 2)
+    want = I8.linear_int8(q, I8.quantize_act_int8(x))
+    monkeypatch.setattr(lib, "_raw_stream", None)
+    monkeypatch.setattr(lib, "_empty_strided_cuda", None)
+    monkeypatch.setattr(lib, "current_index", torch.cuda.current_device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert lib.raw_stream(0) == side.cuda_stream
+        got = I8.linear_int8(q, I8.quantize_act_int8(x))
+    side.synchronize()
+    assert torch.equal(got, want)

@@ -282,3 +282,27 @@ def test_checkpoint_names_its_layout(tmp_path):
         assert label(a) == want
         io.requant_gdn(a, b)
         assert label(b) == after
+
+
+_WITHOUT = """
+import torch
+for holder, name in ((torch._C, "_cuda_getDevice"), (torch._C, "_cuda_getCurrentRawStream"),
+                     (torch._C._dynamo.guards, "_empty_strided_cuda")):
+    if hasattr(holder, name):
+        delattr(holder, name)
+import velogb10_b200.engine.device_sampler, velogb10_b200.models.runtime, velogb10_b200.parallel.comm
+from velogb10_b200.ops import int8, lib
+assert lib._raw_stream is None and lib._empty_strided_cuda is None and lib.current_index is torch.cuda.current_device
+t = lib.empty_beside(torch.zeros(2), (3, 5), (16, 1), torch.int8)
+assert t.shape == (3, 5) and t.stride() == (16, 1) and t.dtype == torch.int8
+print("imported")
+"""
+
+
+def test_imports_without_pytorchs_private_calls():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _WITHOUT], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "imported" in r.stdout, r.stderr[-2000:]

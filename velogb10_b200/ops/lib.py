@@ -55,20 +55,30 @@ def stream() -> c_void_p:
     return c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _private(path: str):
+    """A function of PyTorch's own runtime by its dotted name under ``torch._C``; None where this build or release has none."""
+    obj = torch._C
+    for part in path.split("."):
+        obj = getattr(obj, part, None)
+    return obj
+
+
+# Three calls that PyTorch's own compiled code makes, with the public ones where a build lacks them. They matter in a chain of
+# 5 us kernels: 0.1 us instead of the 2 - 3 us of building a ``torch.cuda.Stream`` object; the current device without the
+# lazy-initialisation check (0.1 us of 0.2); memory without argument parsing and dispatch (0.8 us instead of 1.5).
+_raw_stream = _private("_cuda_getCurrentRawStream")
+current_index = _private("_cuda_getDevice") or torch.cuda.current_device
+_empty_strided_cuda = _private("_dynamo.guards._empty_strided_cuda")
+
+
 def raw_stream(index: int) -> int:
-    """Current stream of device ``index`` as an integer. The call PyTorch's own compiled kernels use: 0.1 us instead of the
-    2 - 3 us of building a ``torch.cuda.Stream`` object, which counts in a chain of 5 us kernels."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-current_index = torch._C._cuda_getDevice        # current device, without the lazy-initialisation check (0.1 us of 0.2)
-_empty_strided_cuda = torch._C._dynamo.guards._empty_strided_cuda
+    """Current stream of device ``index`` as an integer."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def empty_beside(like: torch.Tensor, shape, strides, dtype: torch.dtype) -> torch.Tensor:
-    """Uninitialised tensor on ``like``'s device. On the current CUDA device by the call PyTorch's own compiled code makes,
-    which takes the same memory but skips argument parsing and dispatch: 0.8 us instead of 1.5."""
-    if like.is_cuda and like.get_device() == current_index():
+    """Uninitialised tensor on ``like``'s device."""
+    if like.is_cuda and _empty_strided_cuda is not None and like.get_device() == current_index():
         return _empty_strided_cuda(shape, strides, dtype)
     return torch.empty_strided(shape, strides, dtype=dtype, device=like.device)
 
