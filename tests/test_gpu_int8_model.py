@@ -107,3 +107,25 @@ def test_batch_verify_and_graph_are_bitwise_sequential():
     gm.replay_decode(firsts, pos, [0, 1, 2, 3])
     torch.cuda.synchronize()
     assert gm.ws.out_tok[:4].tolist() == batch.argmax(-1).tolist()
+
+
+def test_gates_cover_int8_linears(capsys):
+    """The batch-invariance gate and the GEMM probe name the formats they ran; an int8 linear that broke must fail the gate."""
+    import json
+    from velogb10_b200 import gates
+    from velogb10_b200.models.runtime import GpuModel
+    cfg, w = _build()
+    gm = GpuModel(w, keep_canonical=True)
+    int8 = [q for _, q in w.linears() if q.fmt == "int8"]
+    assert gates.gate_binv(gm, cfg) == 0
+    out = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert out["formats"]["int8"] == min(12, len(int8)) and out["formats"]["nvfp4"] > 0 and out["rel_l2"] < 1e-3, out
+    assert gates.probe_gemm(gm, cfg) == 0
+    rows = json.loads(capsys.readouterr().out.strip().splitlines()[-1])["rows"]
+    assert {r["format"] for r in rows} >= {"int8", "nvfp4"} and all(r["us"] > 0 and r["GBs"] > 0 for r in rows)
+    scale = int8[0].row_scale
+    int8[0].row_scale = scale * torch.where(torch.arange(scale.numel(), device=scale.device) % 2 == 0, 1.0, 1.1)
+    deq = int8[0].dequant
+    int8[0].dequant = lambda dtype=torch.bfloat16: (int8[0].codes.float() * scale[:, None]).to(dtype)     # plain reference kept
+    assert gates.gate_binv(gm, cfg) == 1
+    int8[0].dequant = deq

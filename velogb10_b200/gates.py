@@ -154,27 +154,43 @@ def gate_state(runner, cfg) -> int:
     return _emit("state", ok)
 
 
+def _gemm_sites(runner, per_format: int):
+    """Up to ``per_format`` dense linears of every weight format the CUDA runtime multiplies with."""
+    seen: Dict[str, int] = {}
+    for name, q in runner.w.linears():
+        if (q.kernel is None and q.fmt != "int8") or q.experts > 1 or seen.get(q.fmt, 0) >= per_format:
+            continue
+        seen[q.fmt] = seen.get(q.fmt, 0) + 1
+        yield name, q
+
+
 def gate_binv(runner, cfg) -> int:
     """Every GEMM site: column 0 at widths 1..16 has the bits of width 1; result close to the dequantised
-    reference (CUDA runtime only)."""
+    reference (CUDA runtime only). int8 linears run on rows quantised at each width; their reference takes the values
+    the codes stand for."""
     if not hasattr(runner, "dev"):
         return _emit("binv", True, note="oracle computes every column independently")
     from .ops import gemm as G
-    worst, sites, bad = 0.0, 0, []
-    for name, q in runner.w.linears():
-        if q.kernel is None or q.experts > 1 or sites >= 12:
-            continue
-        sites += 1
+    from .ops import int8 as I8
+    worst, bad, formats = 0.0, [], {}
+    for name, q in _gemm_sites(runner, 12):
+        formats[q.fmt] = formats.get(q.fmt, 0) + 1
         x = (torch.randn(16, q.k, device=runner.dev) * 0.5).to(torch.float16)
-        base = G.linear(q, x, 1, out_f32=True)[0].clone()
+        if q.fmt == "int8":
+            run = lambda n: I8.linear_int8(q, I8.quantize_act_int8(x, n), out_f32=True)      # noqa: E731
+            x_ref = I8.dequantize_act_int8(I8.quantize_act_int8(x, 1), dtype=torch.float32)
+        else:
+            run = lambda n: G.linear(q, x, n, out_f32=True)                                   # noqa: E731
+            x_ref = x[:1].float()
+        base = run(1)[0].clone()
         for n in range(2, 17):
-            if not torch.equal(G.linear(q, x, n, out_f32=True)[0], base):
+            if not torch.equal(run(n)[0], base):
                 bad.append((name, n))
                 break
         if q.packed is not None or q.codes is not None or q.w is not None:
-            ref = x[:1].float() @ q.dequant(torch.float32).t()
+            ref = x_ref @ q.dequant(torch.float32).t()
             worst = max(worst, float((base - ref[0]).norm() / ref.norm().clamp(min=1e-9)))
-    return _emit("binv", not bad and worst < 0.01, sites=sites, mismatches=bad[:4], rel_l2=worst)
+    return _emit("binv", not bad and worst < 0.01, sites=sum(formats.values()), formats=formats, mismatches=bad[:4], rel_l2=worst)
 
 
 def _stream(runner, cfg, prompt, n_new, policy, params=GREEDY, max_seq=512, **kw):
@@ -374,24 +390,25 @@ def probe_gemm(runner, cfg, sweep: bool = False) -> int:
     if not hasattr(runner, "dev"):
         return 2
     from .ops import gemm as G
+    from .ops import int8 as I8
     rows = []
-    for name, q in runner.w.linears():
-        if q.kernel is None or q.experts > 1:
-            continue
+    for name, q in _gemm_sites(runner, 8 if sweep else 12):
         x = (torch.randn(16, q.k, device=runner.dev) * 0.5).to(torch.float16)
+        if q.fmt == "int8":                       # the product alone: its input comes quantised from the norm or SwiGLU
+            act = I8.quantize_act_int8(x)
+            run, nbytes = (lambda n: I8.linear_int8(q, act, n)), q.codes.numel()
+        else:
+            run, nbytes = (lambda n: G.linear(q, x, n)), q.kernel.wt.numel()
         for n in ([1, 2, 4, 8, 16] if sweep else [1]):
-            G.linear(q, x, n)
+            run(n)
             e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             e0.record()
             for _ in range(5):
-                G.linear(q, x, n)
+                run(n)
             e1.record()
             torch.cuda.synchronize()
             us = e0.elapsed_time(e1) * 200
-            rows.append({"site": name, "m": q.m, "k": q.k, "n": n, "us": us,
-                         "GBs": q.kernel.wt.numel() / us / 1e3})
-        if len(rows) >= (40 if sweep else 12):
-            break
+            rows.append({"site": name, "format": q.fmt, "m": q.m, "k": q.k, "n": n, "us": us, "GBs": nbytes / us / 1e3})
     return _emit("probe-gemm", True, rows=rows)
 
 
