@@ -129,3 +129,24 @@ def test_gates_cover_int8_linears(capsys):
     int8[0].dequant = lambda dtype=torch.bfloat16: (int8[0].codes.float() * scale[:, None]).to(dtype)     # plain reference kept
     assert gates.gate_binv(gm, cfg) == 1
     int8[0].dequant = deq
+
+
+def test_no_f16_rows_beside_int8_rows(monkeypatch):
+    """A dense layer's norms and SwiGLU hand int8 rows to their only reader: no f16 copy is written, no buffer for one is held.
+    The range probe reads the copy, so it gets one, with the same logits."""
+    from velogb10_b200.models import runtime
+    cfg, w = _build()
+    asked, norm = [], runtime.I8.add_rmsnorm_int8
+    monkeypatch.setattr(runtime.I8, "add_rmsnorm_int8", lambda *a, **k: asked.append(k.get("out16")) or norm(*a, **k))
+    gm = runtime.GpuModel(w, keep_canonical=True)
+    gm.alloc_state(2, 2 + 17, 256)
+    prompt = _prompt(cfg, 40)
+    want = gm.prefill(1, prompt)[0].clone()
+    gm.decode([3], [40], [1])
+    assert len(asked) == 4 * cfg.num_layers and all(o is None for o in asked)
+    kept = {L.attn.o.k if L.attn is not None else L.gdn.out.k for L in w.layers}          # mixer outputs are f16
+    assert set(gm.ws._a16) | set(gm.ws_prefill._a16) == kept
+    gm.zero_slot(1)
+    gm.cap_debug, asked[:] = True, []
+    assert torch.equal(gm.prefill(1, prompt)[0], want)
+    assert all(o is not None for o in asked)

@@ -397,7 +397,7 @@ class GpuModel:
         return self.use_fp4 and n <= 16 and getattr(q, "kernel4", None) is not None
 
     def _norm(self, ws: Workspace, delta, w: torch.Tensor, n: int, q: Optional[QLinear] = None):
-        """Residual add + RMSNorm into ``ws.xn16``; at decode widths the same kernel also emits the FP4
+        """Residual add + RMSNorm into ``ws.xn16`` (or int8 rows, below); at decode widths the same kernel also emits the FP4
         activation series, returned for the linears that read this input. When the preceding row-parallel
         linear only pushed its partial rows (``self._pending_ar``), the kernel also performs the
         tensor-parallel sum. When the linear ``q`` that reads the result has int8 weights, the same kernel emits
@@ -410,16 +410,17 @@ class GpuModel:
                 return I8.add_rmsnorm_int8(ws.x, None, w, self.cfg.rms_eps, n, out=ws.i8(ws.x.shape[1]))
             return act
         if q is not None and q.fmt == "int8":
-            return I8.add_rmsnorm_int8(ws.x, delta, w, self.cfg.rms_eps, n, out=ws.i8(ws.x.shape[1]), out16=ws.xn16)
+            return I8.add_rmsnorm_int8(ws.x, delta, w, self.cfg.rms_eps, n, out=ws.i8(ws.x.shape[1]),
+                                       out16=ws.xn16 if self.cap_debug else None)     # nothing else reads the f16 rows
         if self.use_fp4 and n <= 16 and ws.x.shape[1] % 16 == 0:
             return G.add_rmsnorm_fp4(ws.x, delta, w, self.cfg.rms_eps, n, out16=ws.xn16)
         K.add_rmsnorm(ws.x, delta, w, self.cfg.rms_eps, n, out16=ws.xn16)
         return None
 
-    def _linear(self, q: QLinear, x16: torch.Tensor, n: int, out: torch.Tensor, act=None, out_f32: bool = False,
+    def _linear(self, q: QLinear, x16: Optional[torch.Tensor], n: int, out: torch.Tensor, act=None, out_f32: bool = False,
                 comm=None, ws: Optional[Workspace] = None, tag: str = ""):
-        """``act``: the input already quantised for this linear's path (FP4 series or int8 rows), else it is made here
-        (int8: into buffers of ``ws``, or of the call)."""
+        """``act``: the input already quantised for this linear's path (FP4 series or int8 rows; ``x16`` may then be None for
+        int8), else it is made here (int8: into buffers of ``ws``, or of the call)."""
         if q.fmt == "int8":
             assert comm is None
             if not isinstance(act, I8.Int8Act):
@@ -432,7 +433,7 @@ class GpuModel:
         else:
             G.linear(q, x16, n, out=out, out_f32=out_f32, comm=comm)
 
-    def _row_parallel(self, q: QLinear, x16: torch.Tensor, n: int, out: torch.Tensor, reduce: bool = True, act=None,
+    def _row_parallel(self, q: QLinear, x16: Optional[torch.Tensor], n: int, out: torch.Tensor, reduce: bool = True, act=None,
                       ws: Optional[Workspace] = None, tag: str = ""):
         """Row-parallel linear + tensor-parallel sum. For decode / verify widths the reduction is fused into
         the GEMM epilogue (peer-memory pushes + flags inside the same kernel); longer inputs run the GEMM and
@@ -576,11 +577,11 @@ class GpuModel:
         stream must not share them with the main stream's producers)."""
         gu = ws.wide[:, :M.gate_up.m]
         self._linear(M.gate_up, ws.xn16, n, gu, act=act, ws=ws, tag=buf_tag)
-        a16 = ws.a16(M.down.k)
         if M.down.fmt == "int8":
             act_d = I8.swiglu_int8(gu, n, M.inter, out=ws.i8(M.inter, buf_tag))
-            self._row_parallel(M.down, a16, n, out, reduce, act=act_d)
+            self._row_parallel(M.down, None, n, out, reduce, act=act_d)
             return
+        a16 = ws.a16(M.down.k)
         if self._fp4_ok(M.down, n) and M.inter % 8 == 0:
             bufs = G.fp4_buffers(self.dev, ((M.inter + 255) // 256) * 256, tag=buf_tag) if buf_tag else None
             act_d = G.swiglu_fp4(gu, n, M.inter, bufs=bufs)
