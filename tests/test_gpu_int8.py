@@ -598,3 +598,21 @@ def test_without_pytorchs_private_calls(monkeypatch):
         got = I8.linear_int8(q, I8.quantize_act_int8(x))
     side.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("eps", [2.0 ** -100, 1e-12, 1.0, 2.0 ** 127])
+@pytest.mark.parametrize("k", [64, 67, 20000])
+def test_norm_over_the_range_of_eps(eps, k):
+    """Zero rows, rows whose squares leave fp32 at the lower end, ordinary ones; the largest eps leaves only rows of 0."""
+    from velogb10_b200.ops import int8 as I8
+    x = _randn((5, k), k, BF)
+    for r, e in enumerate((-140, -60, -49, 0)):
+        x[r] = (x[r].double() * 2.0 ** e).to(BF)
+    x[4] = 0
+    w = _randn((k,), 1) * 0.2
+    act = I8.add_rmsnorm_int8(x, None, w, eps)
+    # subnormal inputs count as zero (less than 2^-126 of eps^(1/2) or more)
+    y = torch.where(x.double().abs() < 2.0 ** -126, 0.0, x.double())
+    y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * (1 + w.double())
+    _check_rows(act, y, 5, 27 * 2.0 ** -24, (eps, k))
+    assert float(act.scale[4]) == FLOOR and act.scale.isfinite().all()

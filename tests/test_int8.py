@@ -306,3 +306,10 @@ def test_imports_without_pytorchs_private_calls():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", _WITHOUT], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "imported" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("eps", [1e-46, 2.0 ** -127, 2.0 ** -101, 1e39, float("inf"), -1e-6])
+def test_eps_outside_fp32(eps):
+    """An eps that fp32 does not hold: zero rows would become NaN, or all rows zero."""
+    with pytest.raises(KernelError, match="eps"):
+        I8.add_rmsnorm_int8(torch.zeros(2, 8, dtype=BF), None, torch.ones(8), eps)

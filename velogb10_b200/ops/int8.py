@@ -28,6 +28,8 @@ from .lib import KernelError, c_float, c_int, c_ll, c_void_p, empty_beside as _e
 
 MAX_K = 131071                 # 128 * 128 * K must stay below 2^31
 MAX_ROWS = 1 << 27
+# fp32 squares below 2^-126 flush to zero: beside an eps of 2^-100 that is 2^-26 of mean + eps; a smaller one may become zero itself
+EPS_MIN, EPS_MAX = 2.0 ** -100, 2.0 ** 127
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _BF16, _INT8 = (torch.bfloat16,), (torch.int8,)
 
@@ -177,8 +179,8 @@ def add_rmsnorm_int8(res: torch.Tensor, delta: Optional[torch.Tensor], w: torch.
     ``plus_one``) quantised; the normed rows also go to ``out16`` (f16, saturating) when it is given."""
     n, h, ld = _input(res, "res", _BF16, n)
     dev = res.get_device()
-    if not eps > 0.0:
-        raise KernelError(f"eps must be positive, got {eps}")
+    if not EPS_MIN <= eps <= EPS_MAX:
+        raise KernelError(f"eps must be in 2^-100 .. 2^127, got {eps}")
     out, ldq = _out(out, n, h, res)
     ldd = ldo = 0
     if delta is not None:
