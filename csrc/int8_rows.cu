@@ -693,10 +693,27 @@ __global__ void __launch_bounds__(256) dequant_int8_loose_kernel(const signed ch
 // with 212); two teams without weights want a third slot.
 constexpr int RING_BYTES = 200 * 1024, RING_TEAM_BYTES = 212 * 1024;
 constexpr int RING_PER_SM = 16;                   // blocks per SM
-constexpr int RING_MIN_ROWS = 8;                  // rows per SM from which the ring form pays
-constexpr int RING_MIN_WIDE = 1;                  // the same for rows of more than 8192
+// Rows per SM from which the ring form is taken, by row width in groups (us: row form / ring form):
+//   up to 1024   quantise 5120: 1184 rows 6.5 / 6.8, 1500 8.1 / 7.4, 4096 18.2 / 14.9; norm 5120: 1184 11.8 / 12.5, 2000 17.6 /
+//                18.1, 4096 31.2 / 29.2; SwiGLU 8192: 1184 11.8 / 11.7, 4096 33.3 / 31.0. Below about 3000 elements the row
+//                form is still ahead (norm 2560, 4096 rows: 16.3 / 19.5).
+//   up to 1280   all but the norm: SwiGLU 8704: 600 rows 7.6 / 10.4, 3000 26.6 / 27.2; quantise 8704: 1000 8.6 / 9.6, 3000
+//                21.2 / 21.3, 4096 28.3 / 25.1. Norm 8704: 600 14.2 / 14.0, 4096 74.7 / 57.7.
+//   wider        SwiGLU 17408: 149 rows 6.5 / 6.8, 296 9.0 / 8.5, 333 10.6 / 10.3, 1000 25.6 / 18.2, 4096 96 / 57; 12800: 149
+//                5.4 / 6.1, 600 12.6 / 11.3; quantise 17408: 149 5.4 / 5.0, 4096 77 / 38; norm 17408: 149 11.9 / 9.8, 4096 204 / 90.
+constexpr int RING_MIN_ROWS = 8, RING_MIN_MID = 20, RING_MIN_WIDE = 1;
+constexpr int RING_MID_GROUPS = 1280;
 
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  n = known[dev & 63].load();
+  if (n <= 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev & 63].store(n);
+  return n;
+}
 
 template <int KIND, bool VEC>
 cudaError_t launch_shape(RowParams p, int n, cudaStream_t st) {
@@ -706,9 +723,9 @@ cudaError_t launch_shape(RowParams p, int n, cudaStream_t st) {
   constexpr int lanes = SHIFTED ? 31 : 32;
   auto threads = [&](int parts) { return dim3((groups + parts * lanes - 1) / (parts * lanes) * 32); };
   p.cluster = 1;
-  // many shifted rows without a second input: two groups a thread halve the fixed instructions (4096 x 4111 quantise: 25.3
-  // -> 21.3 us; the norm and SwiGLU lose 8 - 20 % to fewer threads)
-  const bool two = !VEC && KIND <= ROW_F32 && n >= 592;
+  // Many shifted 16-bit rows without a second input: two groups a thread halve the fixed instructions. 592 x 4111 6.0 -> 5.0 us,
+  // 1237 9.2 -> 8.4, 4096 26.7 -> 22.7 (but 800 6.6 -> 7.5); 300 x 4111 3.2 -> 4.2, 4096 x 2051 12.7 -> 14.0, fp32 rows 25.3 -> 26.6.
+  const bool two = SHIFTED && KIND <= ROW_F16 && groups > 16 * lanes && n >= 4 * sm_count();
   if (groups <= 32 * lanes && !two) return launch_pdl(row_int8_kernel<KIND, VEC, 1, false>, dim3(n), threads(1), 0, st, p);
   if (groups <= 64 * lanes) return launch_pdl(row_int8_kernel<KIND, VEC, 2, false>, dim3(n), threads(2), 0, st, p);
   while (p.cluster < MAX_CLUSTER && p.cluster * 64 * lanes < groups) p.cluster *= 2;
@@ -717,15 +734,6 @@ cudaError_t launch_shape(RowParams p, int n, cudaStream_t st) {
       return launch_pdl_cluster(row_int8_kernel<KIND, false, 3, true>, dim3(n * p.cluster), threads(3 * p.cluster), p.cluster, 0, st, p);
   }
   return launch_pdl_cluster(row_int8_kernel<KIND, VEC, 2, true>, dim3(n * p.cluster), threads(2 * p.cluster), p.cluster, 0, st, p);
-}
-
-int sm_count() {
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  n = known[dev & 63].load();
-  if (n <= 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev & 63].store(n);
-  return n;
 }
 
 template <int KIND, int MAXC, int TEAMS>
@@ -761,7 +769,9 @@ int launch_row(const RowParams& p, int n, int esize, cudaStream_t st) {
     if (p.out16) vec = vec && aligned(p.out16, 16) && (n == 1 || p.ldo % 8 == 0);
   }
   const int sms = sm_count(), slot = p.k * esize * ((KIND == ROW_SWIGLU || p.delta) ? 2 : 1), groups = p.k / 8;
-  if (vec && n >= (groups > 1024 ? RING_MIN_WIDE : RING_MIN_ROWS) * sms && slot % 16 == 0 && 2 * slot <= RING_BYTES && groups <= RING_GROUPS) {
+  const int ring_rows = groups <= 1024 ? RING_MIN_ROWS
+                        : KIND != ROW_NORM && groups <= RING_MID_GROUPS ? RING_MIN_MID : RING_MIN_WIDE;
+  if (vec && n >= ring_rows * sms && slot % 16 == 0 && 2 * slot <= RING_BYTES && groups <= RING_GROUPS) {
     if constexpr (KIND == ROW_SWIGLU) {
       if (4 * slot > RING_BYTES && groups > 1024) return launch_ring<KIND, 5, 2>(p, n, slot, sms, st);
     }
