@@ -616,3 +616,34 @@ def test_norm_over_the_range_of_eps(eps, k):
     y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * (1 + w.double())
     _check_rows(act, y, 5, 27 * 2.0 ** -24, (eps, k))
     assert float(act.scale[4]) == FLOOR and act.scale.isfinite().all()
+
+
+@pytest.mark.parametrize("n,k", [(1300, 512), (1200, 5120), (150, 8200), (333, 17408), (149, 20480)])
+def test_rows_of_infinities_and_nan_among_many(n, k):
+    """Forms for many rows: such a row gives scale NaN, codes 0 and an f16 row of NaN, its residual is updated like any other,
+    and its neighbours have the bits they have without it."""
+    from velogb10_b200.ops import int8 as I8, lib
+    res, delta, w = _randn((n, k), 1, BF), _randn((n, k), 2, BF), _randn((k,), 3) * 0.2
+    clean, clean16 = res.clone(), torch.empty((n, k), dtype=F16, device="cuda")
+    want = I8.add_rmsnorm_int8(clean, delta, w, 1e-6, out16=clean16)
+    bad = {0: float("nan"), 1: float("inf"), n // 2: float("-inf"), n - 1: float("nan")}
+    dirty_d = delta.clone()
+    for r, v in bad.items():
+        dirty_d[r, (r * 37) % k] = v
+    x, out16 = res.clone(), torch.zeros((n, k), dtype=F16, device="cuda")
+    act = I8.add_rmsnorm_int8(x, dirty_d, w, 1e-6, out16=out16)
+    good = torch.ones(n, dtype=torch.bool, device="cuda")
+    good[list(bad)] = False
+    assert act.scale[~good].isnan().all() and (act.q[~good] == 0).all() and out16[~good].isnan().all()
+    sums = (res.double() + dirty_d.double()).to(BF)
+    assert torch.equal(x.isnan(), sums.isnan()) and torch.equal(x.nan_to_num(7.0), sums.nan_to_num(7.0))
+    assert torch.equal(act.q[good], want.q[good]) and torch.equal(act.scale[good], want.scale[good]) and torch.equal(out16[good], clean16[good])
+    gu = _randn((n, 2 * k), 4, BF)
+    want = I8.swiglu_int8(gu)
+    for r, v in bad.items():
+        gu[r, (r * 37) % (2 * k)] = v
+    act = I8.swiglu_int8(gu)
+    assert act.scale[~good].isnan().all() and (act.q[~good] == 0).all()
+    assert torch.equal(act.q[good], want.q[good]) and torch.equal(act.scale[good], want.scale[good])
+    torch.cuda.synchronize()
+    lib.check_err_word()
