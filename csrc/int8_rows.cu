@@ -589,7 +589,8 @@ row_int8_ring_kernel(const RowParams p, int n, int slots, int slot_bytes) {
     if (stuck[team]) break;                                // seen by the whole team: set before the barrier
     if (tid == 0 && row + (long long)slots * step < n) fill(slot, j + slots, row + (size_t)slots * step);
     float sum = 0.f;
-    if constexpr (KIND == ROW_NORM) sum = sum_of_blocks<MAXC == 4 ? (RING_GROUPS / 32 + 31) / 32 : 1>(block[it & 1], (k + SUM_BLOCK - 1) / SUM_BLOCK);
+    if constexpr (KIND == ROW_NORM)
+      sum = sum_of_blocks<MAXC == 4 ? (RING_GROUPS / 32 + 31) / 32 : 1>(block[it & 1], (k + SUM_BLOCK - 1) / SUM_BLOCK);
     const RowScale rs = row_scale<KIND>(p, mx, sum);
     shrink_big_row<KIND>(v, mx);
     if (tid == 0) p.scale[row] = rs.s;
@@ -689,7 +690,7 @@ __global__ void __launch_bounds__(256) dequant_int8_loose_kernel(const signed ch
   }
 }
 
-// Ring of all blocks of an SM. More of it leaves too little L1 for the norm's weights (4096 x 17408: 86 us with 200 KB, 94
+// Ring of all blocks of an SM. More of it leaves too little L1 for the norm's weights (4096 x 17408: 89 us with 200 KB, 94
 // with 212); two teams without weights want a third slot.
 constexpr int RING_BYTES = 200 * 1024, RING_TEAM_BYTES = 212 * 1024;
 constexpr int RING_PER_SM = 16;                   // blocks per SM
